@@ -309,9 +309,11 @@ def _plain_fork(st):
     count(page_of, copy & ok, -1)
     count(table, fresh, 1)
     st.length[seq] = torch.where(ok, new, old)
-    to = torch.where(copy & ok, torch.gather(table, 1, last.clamp(max=width - 1)[:, None].long())[:, 0].long(), page_of).clamp(min=0)
+    kept = st.table[0, 0].long()      # a page in use, for requests that copy nothing
+    to = torch.where(copy & ok, torch.gather(table, 1, last.clamp(max=width - 1)[:, None].long())[:, 0].long(), kept)
+    at = torch.where(copy & ok, page_of, kept)
     for x in (st.kc, st.vc, st.ks, st.vs):
-        x[:, to] = x[:, page_of.clamp(min=0)]
+        x[:, to] = x[:, at]
     st.got.copy_(ok)
     return [st.table, st.ref, st.length, st.got, st.kc, st.vc, st.ks, st.vs]
 
