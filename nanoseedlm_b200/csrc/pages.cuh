@@ -1,0 +1,108 @@
+// What the kernels of the paged cache share: element types, rotation of 16 values, rows of descriptors.
+#pragma once
+#include "common.cuh"
+#include "../../include/nslm_pages.h"
+
+namespace nsl {
+
+inline bool known_type(int t) { return t == NSL_F32 || t == NSL_BF16 || t == NSL_F32_BF16; }
+inline int type_bytes(int t) { return t == NSL_BF16 ? 2 : 4; }
+// A row's base and stride: 16-byte steps, and room for the row.
+inline bool rows_ok(const void* p, int stride, int width, int type) { return p && aligned16(p) && stride >= width && ((size_t) stride * type_bytes(type)) % 16 == 0; }
+inline bool rope_ok(const NslRope& r, int hd) {
+    return r.rot == 0 || (r.rot > 0 && r.rot % 16 == 0 && r.rot <= hd && r.inv && (r.layout == NSL_ROPE_HALF || r.layout == NSL_ROPE_INTERLEAVED));
+}
+bool pages_ok(const NslPages* p, const char* who);      // pages.cu
+inline bool layer_ok(const NslPages* p, int layer) { return layer >= 0 && layer < p->n_layer; }
+
+#ifdef __CUDACC__
+template <int TYPE>
+__device__ __forceinline__ void load8(const void* base, size_t at, float* x) {
+    if (TYPE == NSL_BF16) {
+        const uint4 u = *(const uint4*) ((const uint16_t*) base + at);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    } else {
+        const float4 a = *(const float4*) ((const float*) base + at), b = *(const float4*) ((const float*) base + at + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+}
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {      // round to nearest even, lo in bits 0-15
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <int TYPE>
+__device__ __forceinline__ void store8(void* base, size_t at, const float* x) {
+    if (TYPE == NSL_F32) {
+        *(float4*) ((float*) base + at) = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*) ((float*) base + at + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        return;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
+    if (TYPE == NSL_BF16) { *(uint4*) ((uint16_t*) base + at) = make_uint4(w[0], w[1], w[2], w[3]); return; }
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { y[2 * i] = __uint_as_float(w[i] << 16); y[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    store8<NSL_F32>(base, at, y);
+}
+
+// (factor cos a, factor sin a) for a = pos * inv.  The product of an int32 and an f32 has at most 55 significant bits and is
+// reduced to half a turn in f64: an f32 product would be off by pos * inv * 2^-24, 0.06 at a million positions.
+__device__ __forceinline__ float2 rope_angle(int pos, float inv, float factor) {
+    double a = (double) pos * (double) inv;
+    a = fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
+    float sn, cs;
+    sincosf((float) a, &sn, &cs);
+    return make_float2(cs * factor, sn * factor);
+}
+// Groups of 16 of a head's values, read as two runs of 8: group g < rot / 16 is rotated by the pairs 8 g .. 8 g + 7, the others
+// are dims 16 g .. 16 g + 15 as they are.
+__device__ __forceinline__ void rope_runs(const NslRope& r, int g, int* a, int* b) {
+    const bool half = r.layout == NSL_ROPE_HALF && 16 * g < r.rot;
+    *a = half ? 8 * g : 16 * g;
+    *b = half ? 8 * g + r.rot / 2 : 16 * g + 8;
+}
+// x: the two runs; cs: (cos, sin) of the group's 8 pairs.
+__device__ __forceinline__ void rope_turn(int layout, float* x, const float2* cs) {
+    if (layout == NSL_ROPE_HALF) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float u = x[i], w = x[i + 8];
+            x[i] = u * cs[i].x - w * cs[i].y;
+            x[i + 8] = w * cs[i].x + u * cs[i].y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float u = x[2 * i], w = x[2 * i + 1];
+            x[2 * i] = u * cs[i].x - w * cs[i].y;
+            x[2 * i + 1] = w * cs[i].x + u * cs[i].y;
+        }
+    }
+}
+
+// The page of a sequence's position, or -1.
+__device__ __forceinline__ int page_of(const NslPages& p, int seq, int j) {
+    if (seq < 0 || seq >= p.n_seq || j < 0 || j >= p.max_pages) return -1;
+    const int id = p.table[(size_t) seq * p.max_pages + j];
+    return id >= 0 && id < p.n_pages ? id : -1;
+}
+// Of row t: the descriptor that names it, -1 where none does.  All threads of a block call it; `found` is shared memory.
+__device__ __forceinline__ int row_descriptor(const NslSeqRows* seqs, int n_seqs, int t, int* found) {
+    __syncthreads();
+    if (threadIdx.x == 0) *found = -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_seqs; i += blockDim.x) {
+        const NslSeqRows d = seqs[i];
+        if (t >= d.row && t - d.row < d.rows) *found = i;
+    }
+    __syncthreads();
+    return *found;
+}
+#endif
+
+}   // namespace nsl

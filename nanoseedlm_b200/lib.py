@@ -72,6 +72,19 @@ assert C.sizeof(WSlice) == 48 and C.sizeof(MmTile) == 16 and C.sizeof(RouterArgs
 
 _vp, _i, _sz = C.c_void_p, C.c_int, C.c_size_t
 
+
+class NslRope(C.Structure):
+    _fields_ = [("inv", C.c_void_p), ("rot", C.c_int32), ("layout", C.c_int32), ("factor", C.c_float), ("pad", C.c_int32)]
+
+
+class NslPages(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "ks", "vs", "ref", "table", "len", "work")] + \
+               [(n, C.c_int32) for n in ("n_layer", "n_pages", "n_kv", "hd", "page", "n_seq", "max_pages", "pad")]
+
+
+assert C.sizeof(NslRope) == 24 and C.sizeof(NslPages) == 96
+
+
 # name -> (restype, argtypes): every symbol include/nslm_kernels.h declares
 PROTOTYPES = {
     "kc_mv": (None, [_vp, _i, WSlice, _i, _i, _vp, _i, _vp, _i, _i, _i, _vp]),
@@ -190,6 +203,18 @@ PROTOTYPES = {
     "nsl_xcache_layer_start": (_i, [_vp, _vp, _i, _i]),
     "nsl_xcache_stats": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
     "nsl_xcache_set_ops": (None, [_vp]),
+    # include/nslm_pages.h
+    "nsl_rope_freqs": (_i, [_i, _i, C.c_double, C.c_double, _i, C.c_double, C.c_double, _vp, _vp]),
+    "nsl_rope": (None, [_vp, NslRope, _i, _i, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _i, _vp, _i]),
+    "nsl_pages_append": (None, [_vp, _vp, _i, NslRope, _i, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _i]),
+    "nsl_pages_read": (None, [_vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _i]),
+    "nsl_pages_attn_work": (_sz, []),
+    "nsl_pages_attn": (None, [_vp, _vp, _i, _i, _vp, _i, _i, C.c_float, _i, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
+    "nsl_pages_extend": (None, [_vp, _vp, _vp, _i, _vp]),
+    "nsl_pages_fork": (None, [_vp, _vp, _vp, _i]),
+    "nsl_pages_trim": (None, [_vp, _vp, _vp, _i]),
+    "nsl_pages_compact": (None, [_vp, _vp]),
+    "nsl_pages_copy": (None, [_vp, _vp, _vp, _i]),
 }
 
 _lib = None
