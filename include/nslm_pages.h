@@ -84,11 +84,14 @@ void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void
  * bf16 (o_type NSL_BF16 or NSL_F32_BF16).  Positions without a page are left out; a row that nothing is left for gives zeros.
  * Queries take part with 11 significant bits (bf16 values exactly), weights with 11, sums in f32.
  * max_rows: no descriptor has more rows (rows beyond it are left as they are).  work: nsl_pages_attn_work() bytes of device
- * memory, 16-byte aligned, zero before its first call; calls that share it run one behind the other, captured ones too.
+ * memory, 16-byte aligned, no initial contents; calls that share it run one behind the other, captured ones too.
  * The steps' keys are dealt evenly to the blocks, so a row alone and in a batch may differ in the order of its f32 sums. */
 size_t nsl_pages_attn_work(void);
 void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, const void* q, int q_stride, int n_head, float scale, int window,
                     const NslSeqRows* seqs, int n_seqs, int max_rows, int T, int o_type, void* o, int o_stride, void* work);
+/* 0, or the code of the first bounded device-side wait that ran out in an attention block since the last call (1 a fetch waiting
+ * for a free stage, 2 a computing warp waiting for a full one); the rows of such a block are not valid.  Call after synchronising. */
+int nsl_pages_attn_status(void);
 
 /* ---- management: device lists, at most NSL_PAGES_LIST entries a call; the calls on a pool run one behind the other -------- */
 #define NSL_PAGES_LIST 1024

@@ -1,19 +1,8 @@
 // Attention of ragged rows over the paged 8-bit cache (nsl_pages_attn).
-#include <math.h>
-
-#include "pages.cuh"
+#include "pages_attn.cuh"
 #include "seed_block.cuh"
 
 namespace nsl {
-
-struct PagesAttn {
-    NslPages p;
-    const void* q;
-    void* o;
-    const NslSeqRows* seqs;
-    float scale;
-    int q_type, q_stride, o_type, o_stride, n_head, layer, window, n_seqs, max_rows, T;
-};
 
 // One block per (head, row): 128 keys at a time, a thread a key for the scores, a thread a dim for the values; the running
 // maximum and sum in f32.  Right for every call, no more.
@@ -28,7 +17,7 @@ __global__ void __launch_bounds__(SIMPLE) pages_attn_simple_kernel(PagesAttn a) 
     const int di = row_descriptor(a.seqs, a.n_seqs, t, &found);
     if (di < 0) return;
     const NslSeqRows d = a.seqs[di];
-    if (t - d.row >= a.max_rows) return;
+    if (t - d.row >= a.max_rows || row_span(a, di).rows * (a.n_head / p.n_kv) <= 16) return;      // few columns: pages_attn_few.cu
     const int pos = d.pos + (t - d.row), k1 = min(pos + 1, p.max_pages * p.page), k0 = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     if (tid < p.hd) {
         const size_t at = (size_t) t * a.q_stride + (size_t) h * p.hd + tid;
@@ -81,13 +70,95 @@ __global__ void __launch_bounds__(SIMPLE) pages_attn_simple_kernel(PagesAttn a) 
     else ((float*) a.o)[at] = o;
 }
 
+// An item's states joined.  Block (b, y): the item that block b of the first pass leaves unfinished, columns 2 y and 2 y + 1; a warp takes
+// every fourth state of a column, four dims a lane (HD = 64: half the lanes).
+constexpr int MERGE_THREADS = 256, MERGE_EACH = MERGE_THREADS / 32 / 2;
+template <int HD>
+__global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a, int most_cols) {
+    constexpr int STATE = PATTN_STATE<HD>;
+    __shared__ float4 sum[MERGE_THREADS / 32][32];
+    __shared__ float stat[MERGE_THREADS / 32][3];
+    grid_dependents_go();
+    grid_dependency_wait();
+    const int4 rec = a.rec[blockIdx.x];
+    const int parts = rec.x & 0xFFFF, kvh = rec.x >> 16, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = 2 * (int) blockIdx.y + warp / MERGE_EACH, turn = warp % MERGE_EACH;
+    if (parts == 0 || 2 * (int) blockIdx.y >= rec.w) return;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float m = -INFINITY, mo = -INFINITY, l = 0.0f;
+    auto state = [&](int i) { return a.part + ((size_t) (2 * ((int) blockIdx.x + i) + (i == 0)) * most_cols + col) * STATE; };
+    if (col < rec.w) {
+        // the maxima over this warp's states, a state a lane; then the sums
+        for (int i = turn + MERGE_EACH * lane; i < parts; i += MERGE_EACH * 32) { m = fmaxf(m, state(i)[HD]); mo = fmaxf(mo, state(i)[HD + 2]); }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) { m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x)); mo = fmaxf(mo, __shfl_xor_sync(0xFFFFFFFFu, mo, x)); }
+        const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
+#pragma unroll 8
+        for (int i = turn; i < parts; i += MERGE_EACH) {
+            const float* st = state(i);
+            const float w = pa_ex2(st[HD + 2] - mos);
+            l = fmaf(st[HD + 1], pa_ex2(st[HD] - ms), l);
+            if (4 * lane < HD) {
+                const float4 v = *(const float4*) (st + 4 * lane);
+                o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
+            }
+        }
+    }
+    sum[warp][lane] = o;
+    if (lane == 0) { stat[warp][0] = m; stat[warp][1] = l; stat[warp][2] = mo; }
+    __syncthreads();
+    if (turn || col >= rec.w || 4 * lane >= HD) return;
+    for (int w = 1; w < MERGE_EACH; ++w) { m = fmaxf(m, stat[warp + w][0]); mo = fmaxf(mo, stat[warp + w][2]); }
+    const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < MERGE_EACH; ++w) {
+        const float4 v = sum[warp + w][lane];
+        const float by = pa_ex2(stat[warp + w][2] - mos);
+        l = fmaf(stat[warp + w][1], pa_ex2(stat[warp + w][0] - ms), l);
+        o.x = fmaf(v.x, by, o.x); o.y = fmaf(v.y, by, o.y); o.z = fmaf(v.z, by, o.z); o.w = fmaf(v.w, by, o.w);
+    }
+    const int group = a.n_head / a.p.n_kv, c = rec.z + col;
+    const float f = pattn_factor(m, l, mo);
+    const size_t at = (size_t) (rec.y + c / group) * a.o_stride + (size_t) (kvh * group + c % group) * HD + 4 * lane;
+    const uint32_t lo = bf16_pair(o.x * f, o.y * f), hi = bf16_pair(o.z * f, o.w * f);
+    if (a.o_type == NSL_BF16) *(uint2*) ((uint16_t*) a.o + at) = make_uint2(lo, hi);
+    else *(float4*) ((float*) a.o + at) = make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xFFFF0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xFFFF0000u));
+}
+
+void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks, int most_cols) {
+    const dim3 grid((unsigned) blocks, (unsigned) (most_cols + 1) / 2);
+    if (a.p.hd == 128) launch(pattn_merge_kernel<128>, grid, MERGE_THREADS, 0, s, a, most_cols);
+    else launch(pattn_merge_kernel<64>, grid, MERGE_THREADS, 0, s, a, most_cols);
+}
+
+// Encoded at every call: a map is 128 bytes of the launch's arguments, and a pool's buffers are the caller's.
+bool pattn_map(CUtensorMap* tm, const NslPages& p, const int8_t* codes) {
+    typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                               CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* f = NULL;
+        cudaDriverEntryPointQueryResult r;
+        return cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) == cudaSuccess && r == cudaDriverEntryPointSuccess ? (Encode) f : (Encode) NULL;
+    }();
+    const cuuint64_t rows = (cuuint64_t) p.n_layer * p.n_pages * p.n_kv * p.page;
+    if (!encode || rows > 0x7FFFFFFFull) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t) p.hd, rows}, strides[1] = {(cuuint64_t) p.hd};
+    const cuuint32_t box[2] = {(cuuint32_t) p.hd, (cuuint32_t) (p.page < 64 ? p.page : 64)}, step[2] = {1, 1};
+    return encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*) codes, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  p.hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }   // namespace nsl
 
 using namespace nsl;
 
 extern "C" {
 
-size_t nsl_pages_attn_work(void) { return 1 << 20; }
+// A record and two partial states a block, of 16 columns each.
+size_t nsl_pages_attn_work(void) { return (size_t) pattn_blocks() * (16 + 2 * 16 * PATTN_STATE<128> * 4); }
+
+int nsl_pages_attn_status(void) { return pattn_few_status(); }
 
 void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, const void* q, int q_stride, int n_head, float scale, int window,
                     const NslSeqRows* seqs, int n_seqs, int max_rows, int T, int o_type, void* o, int o_stride, void* work) {
@@ -99,10 +170,20 @@ void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, co
                   q_type, o_type, n_head, p->n_kv, n_seqs);
         return;
     }
+    CUtensorMap tk, tv;
+    if (!pattn_map(&tk, *p, p->k) || !pattn_map(&tv, *p, p->v)) { set_error("nsl_pages_attn: no tensor map for the pool's codes"); return; }
     FollowScope follow;
-    const PagesAttn a = {*p, q, o, seqs, scale, q_type, q_stride, o_type, o_stride, n_head, layer, window, n_seqs, max_rows, T};
-    launch(pages_attn_simple_kernel, dim3((unsigned) n_head, (unsigned) T), SIMPLE, 0, s, a);
-    count_launch();
+    PagesAttn a;
+    a.p = *p; a.q = q; a.o = o; a.seqs = seqs;
+    a.rec = (int4*) work;
+    a.part = (float*) ((char*) work + 16 * (size_t) pattn_blocks());
+    a.scale = scale; a.q_type = q_type; a.q_stride = q_stride; a.o_type = o_type; a.o_stride = o_stride;
+    a.n_head = n_head; a.layer = layer; a.window = window; a.n_seqs = n_seqs; a.max_rows = max_rows; a.T = T;
+    if (n_head / p->n_kv <= 16) launch_pattn_few(s, a, tk, tv);
+    if ((long long) (n_head / p->n_kv) * max_rows > 16) {
+        launch(pages_attn_simple_kernel, dim3((unsigned) n_head, (unsigned) T), SIMPLE, 0, s, a);
+        count_launch();
+    }
 }
 
 }   // extern "C"

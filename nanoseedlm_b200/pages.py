@@ -116,7 +116,7 @@ class PagePool:
         self.lib, self.device = L.load(), device
         self.k, self.v, self.ks, self.vs, self.ref, self.table, self.length = k, v, ks, vs, ref, table, length
         self.work = torch.empty(4 + 3 * shape[1], dtype=torch.int32, device=device)
-        self.attn_work = torch.zeros(self.lib.nsl_pages_attn_work() // 4, dtype=torch.int32, device=device)
+        self.attn_work = torch.empty(self.lib.nsl_pages_attn_work() // 4, dtype=torch.int32, device=device)
         self.kv, self.hd, self.page = shape[2], shape[4], shape[3]
         self.struct = L.NslPages(*(t.data_ptr() for t in (k, v, ks, vs, ref, table, length, self.work)), shape[0], shape[1], shape[2], shape[4], shape[3], table.shape[0],
                                table.shape[1], 0)
@@ -160,7 +160,7 @@ class PagePool:
 
     def attn(self, layer, q, rows, out, max_rows, scale=None, window=0, work=None):
         """Causal attention of q [T][heads][hd] over the sequences' pages -> out (bfloat16, or float32 rounded to bf16).  work: other
-        work memory than the pool's own (int32, zero before its first call), for calls that may run beside one another."""
+        work memory than the pool's own (int32), for calls that may run beside one another."""
         work = self.attn_work if work is None else work
         _here(self.device, q, rows, out, work)
         qs, os = _rows(q, "q"), _rows(out, "out")
