@@ -10,7 +10,6 @@ from . import lib as L
 
 NSL_F32, NSL_BF16, NSL_F32_BF16 = 0, 1, 2
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
-_NULL = C.c_void_p(0)
 
 
 def rope_freqs(rot, theta, kind=ROPE_PLAIN, scale=1.0, ctx=0, beta_fast=32.0, beta_slow=1.0):
@@ -27,73 +26,84 @@ class Rope:
     def __init__(self, inv, interleaved=False, factor=1.0):
         if inv.dtype != torch.float32 or not inv.is_cuda or not inv.is_contiguous() or inv.dim() != 1:
             raise ValueError("inv: a contiguous float32 device vector")
-        self.inv, self.device = inv, inv.device
+        self.inv = inv
         self.struct = L.NslRope(inv.data_ptr(), 2 * inv.numel(), int(interleaved), factor, 0)
 
 
 _NO_ROPE = L.NslRope(0, 0, 0, 1.0, 0)
 
 
+_TYPES = {torch.bfloat16: (NSL_BF16, NSL_BF16), torch.float32: (NSL_F32, NSL_F32_BF16)}
+
+
 def _type(t, rounded=False):
-    if t.dtype == torch.bfloat16:
-        return NSL_BF16
-    if t.dtype == torch.float32:
-        return NSL_F32_BF16 if rounded else NSL_F32
-    raise ValueError(f"{t.dtype}: float32 or bfloat16 rows")
+    try:
+        return _TYPES[t.dtype][rounded]
+    except KeyError:
+        raise ValueError(f"{t.dtype}: float32 or bfloat16 rows") from None
 
 
 def _rows(t, name, like=None):
     """[T][heads][hd] with dense heads: the row stride in elements."""
-    if t.dim() != 3 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
-        raise ValueError(f"{name}: [T][heads][hd] with dense heads, got {tuple(t.shape)} with strides {t.stride()}")
-    if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2]):
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name}: [T][heads][hd], got {tuple(shape)}")
+    rs, hs, es = t.stride()
+    if es != 1 or (shape[1] > 1 and hs != shape[2]):
+        raise ValueError(f"{name}: dense heads, got strides {t.stride()}")
+    if like is not None and (t.dtype != like.dtype or shape[0] != like.shape[0] or shape[2] != like.shape[2]):
         raise ValueError(f"{name}: another type, number of rows or head width than the other rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return rs if shape[0] > 1 else shape[1] * shape[2]
 
 
-def _ints(t, name, width, device):
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device or (t.dim() != 2 or t.shape[1] != width if width else t.dim() != 1):
-        raise ValueError(f"{name}: a contiguous int32 tensor {'[n][%d]' % width if width else '[n]'} on {device}")
-    return t.shape[0]
+def _ints(t, name, width):
+    """A contiguous int32 list [n][width] ([n] for width 0): n."""
+    shape = t.shape
+    if t.dtype != torch.int32 or not t.is_contiguous() or (len(shape) != 2 or shape[1] != width if width else len(shape) != 1):
+        raise ValueError(f"{name}: a contiguous int32 tensor {'[n][%d]' % width if width else '[n]'}")
+    return shape[0]
 
 
-def _here(device, *tensors):
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+def _here(index, *tensors):
+    """All on the device `index`, and that the current one."""
+    if index != torch.cuda.current_device():
+        raise ValueError(f"tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"a tensor on {t.device} among tensors on {device}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"a tensor on {t.device} among tensors on cuda:{index}")
 
 
 def _done():
-    msg = L.last_error()
+    """Raises what the call was refused for."""
+    msg = L.load().nsl_last_error()
     if msg:
-        raise ValueError(msg)
+        raise ValueError(msg.decode())
 
 
-def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+def _stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 def _ptr(t):
-    return C.c_void_p(t.data_ptr()) if t is not None else _NULL
+    return t.data_ptr() if t is not None else None
 
 
 def rope(r, q, k, pos, q_out=None, k_out=None, rounded=False):
     """Rotates the heads of q [T][heads][hd] and k (or None) at positions pos (int32 [T]); in place without outputs.  rounded: float32
     results are rounded to bf16."""
     q_out, k_out = q if q_out is None else q_out, k if k_out is None else k_out
-    _here(q.device, k, pos, q_out, k_out, r.inv)
-    qs, T, hd = _rows(q, "q"), q.shape[0], q.shape[2]
-    qos = _rows(q_out, "q_out", q)
-    if q_out.shape != q.shape or _ints(pos, "pos", 0, q.device) != T:
+    index = q.get_device()
+    _here(index, k, pos, q_out, k_out, r.inv)
+    qs, (T, heads, hd) = _rows(q, "q"), q.shape
+    qos = qs if q_out is q else _rows(q_out, "q_out", q)
+    if q_out.shape != q.shape or _ints(pos, "pos", 0) != T:
         raise ValueError("q_out: the shape of q; pos: one position a row")
     ks = kos = kv = 0
     if k is not None:
         ks, kos, kv = _rows(k, "k", q), _rows(k_out, "k_out", q), k.shape[1]
         if k_out.shape != k.shape:
             raise ValueError("k_out: the shape of k")
-    L.load().nsl_rope(_stream(), r.struct, _type(q, rounded), hd, _ptr(q), qs, _ptr(q_out), qos, q.shape[1], _ptr(k), ks, _ptr(k_out), kos, kv, _ptr(pos), T)
+    L.load().nsl_rope(_stream(index), r.struct, _type(q, rounded), hd, _ptr(q), qs, _ptr(q_out), qos, heads, _ptr(k), ks, _ptr(k_out), kos, kv, _ptr(pos), T)
     _done()
 
 
@@ -113,11 +123,12 @@ class PagePool:
                 raise ValueError(f"{name}: a contiguous {dt} device tensor {tuple(sh)} on {device}, got {t.dtype} {tuple(t.shape)}")
         if k.dim() != 5 or table.dim() != 2:
             raise ValueError("k: [layers][pages][kv heads][page][hd]; table: [sequences][pages of a sequence]")
-        self.lib, self.device = L.load(), device
+        self.lib, self.device, self.index = L.load(), device, device.index
         self.k, self.v, self.ks, self.vs, self.ref, self.table, self.length = k, v, ks, vs, ref, table, length
         self.work = torch.empty(4 + 3 * shape[1], dtype=torch.int32, device=device)
         self.attn_work = torch.empty(self.lib.nsl_pages_attn_work() // 4, dtype=torch.int32, device=device)
         self.kv, self.hd, self.page = shape[2], shape[4], shape[3]
+        self._heads = (self.kv, self.hd)
         self.struct = L.NslPages(*(t.data_ptr() for t in (k, v, ks, vs, ref, table, length, self.work)), shape[0], shape[1], shape[2], shape[4], shape[3], table.shape[0],
                                table.shape[1], 0)
         self._p = C.byref(self.struct)
@@ -133,71 +144,71 @@ class PagePool:
     def append(self, layer, r, q, k, v, rows, q_out=None, rounded=False):
         """Rotates q (or None; in place without q_out) and k as r says (None: not at all) and stores k, v [T][kv heads][hd] at the
         descriptors' positions."""
-        _here(self.device, q, k, v, rows, q_out, r.inv if r is not None else None)
+        _here(self.index, q, k, v, rows, q_out, r.inv if r is not None else None)
         q_out = q if q_out is None else q_out
         ks, vs, T = _rows(k, "k"), _rows(v, "v", k), k.shape[0]
-        if k.shape[1:] != (self.kv, self.hd) or v.shape != k.shape:
+        if k.shape[1:] != self._heads or v.shape != k.shape:
             raise ValueError(f"k, v: [T][{self.kv}][{self.hd}]")
         qs = qos = heads = 0
         if q is not None:
             qs, qos, heads = _rows(q, "q", k), _rows(q_out, "q_out", k), q.shape[1]
             if q_out.shape != q.shape:
                 raise ValueError("q_out: the shape of q")
-        n = _ints(rows, "rows", 4, self.device)
-        self.lib.nsl_pages_append(_stream(), self._p, layer, r.struct if r is not None else _NO_ROPE, _type(k, rounded), _ptr(q), qs, _ptr(q_out), qos, heads, _ptr(k), ks, _ptr(v), vs,
+        n = _ints(rows, "rows", 4)
+        self.lib.nsl_pages_append(_stream(self.index), self._p, layer, r.struct if r is not None else _NO_ROPE, _type(k, rounded), _ptr(q), qs, _ptr(q_out), qos, heads, _ptr(k), ks, _ptr(v), vs,
                                   _ptr(rows), n, T)
         _done()
 
     def read(self, layer, rows, k_out, v_out, rounded=False):
         """The values at the descriptors' positions -> k_out, v_out [T][kv heads][hd]."""
-        _here(self.device, rows, k_out, v_out)
+        _here(self.index, rows, k_out, v_out)
         ks, vs = _rows(k_out, "k_out"), _rows(v_out, "v_out", k_out)
-        if k_out.shape[1:] != (self.kv, self.hd) or v_out.shape != k_out.shape:
+        if k_out.shape[1:] != self._heads or v_out.shape != k_out.shape:
             raise ValueError(f"k_out, v_out: [T][{self.kv}][{self.hd}]")
-        n = _ints(rows, "rows", 4, self.device)
-        self.lib.nsl_pages_read(_stream(), self._p, layer, _type(k_out, rounded), _ptr(k_out), ks, _ptr(v_out), vs, _ptr(rows), n, k_out.shape[0])
+        n = _ints(rows, "rows", 4)
+        self.lib.nsl_pages_read(_stream(self.index), self._p, layer, _type(k_out, rounded), _ptr(k_out), ks, _ptr(v_out), vs, _ptr(rows), n, k_out.shape[0])
         _done()
 
     def attn(self, layer, q, rows, out, max_rows, scale=None, window=0, work=None):
         """Causal attention of q [T][heads][hd] over the sequences' pages -> out (bfloat16, or float32 rounded to bf16).  work: other
         work memory than the pool's own (int32), for calls that may run beside one another."""
         work = self.attn_work if work is None else work
-        _here(self.device, q, rows, out, work)
+        _here(self.index, q, rows, out, work)
         qs, os = _rows(q, "q"), _rows(out, "out")
         if out.shape != q.shape or q.shape[2] != self.hd:
             raise ValueError(f"q, out: [T][heads][{self.hd}]")
-        if _ints(work, "work", 0, self.device) < self.attn_work.numel():
+        if _ints(work, "work", 0) < self.attn_work.numel():
             raise ValueError(f"work: {self.attn_work.numel()} ints")
-        n = _ints(rows, "rows", 4, self.device)
-        self.lib.nsl_pages_attn(_stream(), self._p, layer, _type(q), _ptr(q), qs, q.shape[1], self.hd ** -0.5 if scale is None else scale, window, _ptr(rows), n, max_rows, q.shape[0],
+        n = _ints(rows, "rows", 4)
+        self.lib.nsl_pages_attn(_stream(self.index), self._p, layer, _type(q), _ptr(q), qs, q.shape[1], self.hd ** -0.5 if scale is None else scale, window, _ptr(rows), n, max_rows, q.shape[0],
                                 _type(out, True), _ptr(out), os, _ptr(work))
         _done()
 
     def extend(self, reqs, got=None):
         """Sequences grow: reqs int32 [n][2] = (sequence, length); got (int32 [n], optional): 1 where served."""
-        _here(self.device, reqs, got)
-        n = _ints(reqs, "reqs", 2, self.device)
-        if got is not None and _ints(got, "got", 0, self.device) < n:
+        _here(self.index, reqs, got)
+        n = _ints(reqs, "reqs", 2)
+        if got is not None and _ints(got, "got", 0) < n:
             raise ValueError("got: one value a request")
-        self.lib.nsl_pages_extend(_stream(), self._p, _ptr(reqs), n, _ptr(got))
+        self.lib.nsl_pages_extend(_stream(self.index), self._p, _ptr(reqs), n, _ptr(got))
         _done()
 
     def fork(self, forks):
         """forks int32 [n][4] = (source, destination, length, 0): the destination shares the source's first positions."""
-        _here(self.device, forks)
-        self.lib.nsl_pages_fork(_stream(), self._p, _ptr(forks), _ints(forks, "forks", 4, self.device))
+        _here(self.index, forks)
+        self.lib.nsl_pages_fork(_stream(self.index), self._p, _ptr(forks), _ints(forks, "forks", 4))
         _done()
 
     def trim(self, reqs):
         """Sequences are cut back: reqs int32 [n][2] = (sequence, length)."""
-        _here(self.device, reqs)
-        self.lib.nsl_pages_trim(_stream(), self._p, _ptr(reqs), _ints(reqs, "reqs", 2, self.device))
+        _here(self.index, reqs)
+        self.lib.nsl_pages_trim(_stream(self.index), self._p, _ptr(reqs), _ints(reqs, "reqs", 2))
         _done()
 
     def compact(self):
         """The pages in use move to the lowest ids; used() says how many there are."""
-        _here(self.device)
-        self.lib.nsl_pages_compact(_stream(), self._p)
+        _here(self.index)
+        self.lib.nsl_pages_compact(_stream(self.index), self._p)
         _done()
 
     def used(self):
@@ -206,6 +217,6 @@ class PagePool:
 
     def copy(self, pairs):
         """Pages pairs[i][0] -> pairs[i][1] (int32 [n][2]), in all layers."""
-        _here(self.device, pairs)
-        self.lib.nsl_pages_copy(_stream(), self._p, _ptr(pairs), _ints(pairs, "pairs", 2, self.device))
+        _here(self.index, pairs)
+        self.lib.nsl_pages_copy(_stream(self.index), self._p, _ptr(pairs), _ints(pairs, "pairs", 2))
         _done()
