@@ -1,77 +1,10 @@
 // Attention of ragged rows over the paged 8-bit cache (nsl_pages_attn).
 #include "pages_attn.cuh"
-#include "seed_block.cuh"
 
 namespace nsl {
 
-// One block per (head, row): 128 keys at a time, a thread a key for the scores, a thread a dim for the values; the running
-// maximum and sum in f32.  Right for every call, no more.
-constexpr int SIMPLE = 128;
-__global__ void __launch_bounds__(SIMPLE) pages_attn_simple_kernel(PagesAttn a) {
-    __shared__ float qs[128], ps[SIMPLE], red[SIMPLE / 32];
-    __shared__ int found;
-    grid_dependents_go();
-    grid_dependency_wait();
-    const NslPages& p = a.p;
-    const int h = blockIdx.x, t = blockIdx.y, tid = threadIdx.x, kvh = h / (a.n_head / p.n_kv);
-    const int di = row_descriptor(a.seqs, a.n_seqs, t, &found);
-    if (di < 0) return;
-    const NslSeqRows d = a.seqs[di];
-    if (t - d.row >= a.max_rows || row_span(a, di).rows * (a.n_head / p.n_kv) <= 16) return;      // few columns: pages_attn_few.cu
-    const int pos = d.pos + (t - d.row), k1 = min(pos + 1, p.max_pages * p.page), k0 = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    if (tid < p.hd) {
-        const size_t at = (size_t) t * a.q_stride + (size_t) h * p.hd + tid;
-        qs[tid] = a.q_type == NSL_BF16 ? __uint_as_float((uint32_t) ((const uint16_t*) a.q)[at] << 16) : ((const float*) a.q)[at];
-    }
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    for (int b = k0; b < k1; b += SIMPLE) {
-        const int key = b + tid;
-        float s = -INFINITY;
-        if (key < k1) {
-            const int id = page_of(p, d.seq, key / p.page);
-            if (id >= 0) {
-                const size_t page_at = ((size_t) a.layer * p.n_pages + id) * p.n_kv + kvh;
-                const char4* row = (const char4*) (p.k + (page_at * p.page + key % p.page) * p.hd);
-                float sum = 0.0f;
-                for (int w = 0; w < p.hd / 4; ++w) {
-                    const char4 c = row[w];
-                    sum += qs[4 * w] * c.x + qs[4 * w + 1] * c.y + qs[4 * w + 2] * c.z + qs[4 * w + 3] * c.w;
-                }
-                s = sum * p.ks[page_at] * a.scale;
-            }
-        }
-        float mx = s;
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-        __syncthreads();
-        if ((tid & 31) == 0) red[tid >> 5] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        mx = fmaxf(mx, m);
-        if (mx == -INFINITY) continue;      // nothing yet; the same for all threads
-        const float cor = expf(m - mx), e = expf(s - mx);
-        m = mx;
-        ps[tid] = e;
-        __syncthreads();
-        l *= cor;
-        acc *= cor;
-        for (int i = 0; i < SIMPLE && b + i < k1; ++i) {
-            l += ps[i];
-            if (ps[i] == 0.0f || tid >= p.hd) continue;
-            const int id = page_of(p, d.seq, (b + i) / p.page);
-            const size_t page_at = ((size_t) a.layer * p.n_pages + id) * p.n_kv + kvh;
-            acc += ps[i] * ((float) p.v[(page_at * p.page + (b + i) % p.page) * p.hd + tid] * p.vs[page_at]);
-        }
-    }
-    if (tid >= p.hd) return;
-    const float o = bf16_round(l > 0.0f ? acc / l : 0.0f);
-    const size_t at = (size_t) t * a.o_stride + (size_t) h * p.hd + tid;
-    if (a.o_type == NSL_BF16) ((uint16_t*) a.o)[at] = bf16_bits(o);
-    else ((float*) a.o)[at] = o;
-}
-
-// An item's states joined.  Block (b, y): the item that block b of the first pass leaves unfinished, columns 2 y and 2 y + 1; a warp takes
-// every fourth state of a column, four dims a lane (HD = 64: half the lanes).
+// An item's states joined.  Block (b, y): the item that block b of the first pass leaves unfinished, every gridDim.y-th pair of its
+// columns; a warp takes every fourth state of a column, four dims a lane (HD = 64: half the lanes).
 constexpr int MERGE_THREADS = 256, MERGE_EACH = MERGE_THREADS / 32 / 2;
 template <int HD>
 __global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a, int most_cols) {
@@ -81,53 +14,57 @@ __global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a,
     grid_dependents_go();
     grid_dependency_wait();
     const int4 rec = a.rec[blockIdx.x];
-    const int parts = rec.x & 0xFFFF, kvh = rec.x >> 16, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = 2 * (int) blockIdx.y + warp / MERGE_EACH, turn = warp % MERGE_EACH;
-    if (parts == 0 || 2 * (int) blockIdx.y >= rec.w) return;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float m = -INFINITY, mo = -INFINITY, l = 0.0f;
-    auto state = [&](int i) { return a.part + ((size_t) (2 * ((int) blockIdx.x + i) + (i == 0)) * most_cols + col) * STATE; };
-    if (col < rec.w) {
-        // the maxima over this warp's states, a state a lane; then the sums
-        for (int i = turn + MERGE_EACH * lane; i < parts; i += MERGE_EACH * 32) { m = fmaxf(m, state(i)[HD]); mo = fmaxf(mo, state(i)[HD + 2]); }
+    const int parts = rec.x & 0xFFFF, kvh = rec.x >> 16, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, turn = warp % MERGE_EACH;
+    if (parts == 0) return;
+    for (int pair = blockIdx.y; 2 * pair < rec.w; pair += gridDim.y) {
+        const int col = 2 * pair + warp / MERGE_EACH;
+        __syncthreads();      // the last pair's sums have been read
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float m = -INFINITY, mo = -INFINITY, l = 0.0f;
+        auto state = [&](int i) { return a.part + ((size_t) (2 * ((int) blockIdx.x + i) + (i == 0)) * most_cols + col) * STATE; };
+        if (col < rec.w) {
+            // the maxima over this warp's states, a state a lane; then the sums
+            for (int i = turn + MERGE_EACH * lane; i < parts; i += MERGE_EACH * 32) { m = fmaxf(m, state(i)[HD]); mo = fmaxf(mo, state(i)[HD + 2]); }
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) { m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x)); mo = fmaxf(mo, __shfl_xor_sync(0xFFFFFFFFu, mo, x)); }
-        const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
+            for (int x = 16; x > 0; x >>= 1) { m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x)); mo = fmaxf(mo, __shfl_xor_sync(0xFFFFFFFFu, mo, x)); }
+            const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
 #pragma unroll 8
-        for (int i = turn; i < parts; i += MERGE_EACH) {
-            const float* st = state(i);
-            const float w = pa_ex2(st[HD + 2] - mos);
-            l = fmaf(st[HD + 1], pa_ex2(st[HD] - ms), l);
-            if (4 * lane < HD) {
-                const float4 v = *(const float4*) (st + 4 * lane);
-                o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
+            for (int i = turn; i < parts; i += MERGE_EACH) {
+                const float* st = state(i);
+                const float w = pa_ex2(st[HD + 2] - mos);
+                l = fmaf(st[HD + 1], pa_ex2(st[HD] - ms), l);
+                if (4 * lane < HD) {
+                    const float4 v = *(const float4*) (st + 4 * lane);
+                    o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
+                }
             }
         }
-    }
-    sum[warp][lane] = o;
-    if (lane == 0) { stat[warp][0] = m; stat[warp][1] = l; stat[warp][2] = mo; }
-    __syncthreads();
-    if (turn || col >= rec.w || 4 * lane >= HD) return;
-    for (int w = 1; w < MERGE_EACH; ++w) { m = fmaxf(m, stat[warp + w][0]); mo = fmaxf(mo, stat[warp + w][2]); }
-    const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
-    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    l = 0.0f;
+        sum[warp][lane] = o;
+        if (lane == 0) { stat[warp][0] = m; stat[warp][1] = l; stat[warp][2] = mo; }
+        __syncthreads();
+        if (turn || col >= rec.w || 4 * lane >= HD) continue;
+        for (int w = 1; w < MERGE_EACH; ++w) { m = fmaxf(m, stat[warp + w][0]); mo = fmaxf(mo, stat[warp + w][2]); }
+        const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
+        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < MERGE_EACH; ++w) {
-        const float4 v = sum[warp + w][lane];
-        const float by = pa_ex2(stat[warp + w][2] - mos);
-        l = fmaf(stat[warp + w][1], pa_ex2(stat[warp + w][0] - ms), l);
-        o.x = fmaf(v.x, by, o.x); o.y = fmaf(v.y, by, o.y); o.z = fmaf(v.z, by, o.z); o.w = fmaf(v.w, by, o.w);
+        for (int w = 0; w < MERGE_EACH; ++w) {
+            const float4 v = sum[warp + w][lane];
+            const float by = pa_ex2(stat[warp + w][2] - mos);
+            l = fmaf(stat[warp + w][1], pa_ex2(stat[warp + w][0] - ms), l);
+            o.x = fmaf(v.x, by, o.x); o.y = fmaf(v.y, by, o.y); o.z = fmaf(v.z, by, o.z); o.w = fmaf(v.w, by, o.w);
+        }
+        const int group = a.n_head / a.p.n_kv, c = rec.z + col;
+        const float f = pattn_factor(m, l, mo);
+        const size_t at = (size_t) (rec.y + c / group) * a.o_stride + (size_t) (kvh * group + c % group) * HD + 4 * lane;
+        const uint32_t lo = bf16_pair(o.x * f, o.y * f), hi = bf16_pair(o.z * f, o.w * f);
+        if (a.o_type == NSL_BF16) *(uint2*) ((uint16_t*) a.o + at) = make_uint2(lo, hi);
+        else *(float4*) ((float*) a.o + at) = make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xFFFF0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xFFFF0000u));
     }
-    const int group = a.n_head / a.p.n_kv, c = rec.z + col;
-    const float f = pattn_factor(m, l, mo);
-    const size_t at = (size_t) (rec.y + c / group) * a.o_stride + (size_t) (kvh * group + c % group) * HD + 4 * lane;
-    const uint32_t lo = bf16_pair(o.x * f, o.y * f), hi = bf16_pair(o.z * f, o.w * f);
-    if (a.o_type == NSL_BF16) *(uint2*) ((uint16_t*) a.o + at) = make_uint2(lo, hi);
-    else *(float4*) ((float*) a.o + at) = make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xFFFF0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xFFFF0000u));
 }
 
 void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks, int most_cols) {
-    const dim3 grid((unsigned) blocks, (unsigned) (most_cols + 1) / 2);
+    const dim3 grid((unsigned) blocks, (unsigned) (most_cols / 2 < 16 ? most_cols / 2 : 16));
     if (a.p.hd == 128) launch(pattn_merge_kernel<128>, grid, MERGE_THREADS, 0, s, a, most_cols);
     else launch(pattn_merge_kernel<64>, grid, MERGE_THREADS, 0, s, a, most_cols);
 }
@@ -155,10 +92,13 @@ using namespace nsl;
 
 extern "C" {
 
-// A record and two partial states a block, of 16 columns each.
-size_t nsl_pages_attn_work(void) { return (size_t) pattn_blocks() * (16 + 2 * 16 * PATTN_STATE<128> * 4); }
+// A record a block, and two states for each of the blocks of either kernel (two an SM of up to PATTN_FEW columns, one of up to PATTN_MANY).
+size_t nsl_pages_attn_work(void) { return (size_t) pattn_blocks() * 16 + (size_t) sm_count() * 2 * PATTN_MANY * PATTN_STATE<128> * 4; }
 
-int nsl_pages_attn_status(void) { return pattn_few_status(); }
+int nsl_pages_attn_status(void) {
+    const int few = pattn_few_status(), many = pattn_many_status();
+    return few ? few : many;
+}
 
 void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, const void* q, int q_stride, int n_head, float scale, int window,
                     const NslSeqRows* seqs, int n_seqs, int max_rows, int T, int o_type, void* o, int o_stride, void* work) {
@@ -179,11 +119,9 @@ void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, co
     a.part = (float*) ((char*) work + 16 * (size_t) pattn_blocks());
     a.scale = scale; a.q_type = q_type; a.q_stride = q_stride; a.o_type = o_type; a.o_stride = o_stride;
     a.n_head = n_head; a.layer = layer; a.window = window; a.n_seqs = n_seqs; a.max_rows = max_rows; a.T = T;
-    if (n_head / p->n_kv <= 16) launch_pattn_few(s, a, tk, tv);
-    if ((long long) (n_head / p->n_kv) * max_rows > 16) {
-        launch(pages_attn_simple_kernel, dim3((unsigned) n_head, (unsigned) T), SIMPLE, 0, s, a);
-        count_launch();
-    }
+    const int group = n_head / p->n_kv, few = group <= PATTN_FEW ? PATTN_FEW : 0;
+    if (few) launch_pattn_few(s, a, tk, tv);
+    if ((long long) group * (max_rows < T ? max_rows : T) > few) launch_pattn_many(s, a, few, tk, tv);
 }
 
 }   // extern "C"

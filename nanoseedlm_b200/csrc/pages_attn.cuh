@@ -21,9 +21,12 @@ struct PagesAttn {
 
 // Blocks of a launch: two an SM (their number fits a record's 16 bits).
 inline int pattn_blocks() { return 2 * sm_count(); }
+constexpr int PATTN_FEW = 16, PATTN_MANY = 256;      // columns of an item
 template <int HD>
 constexpr int PATTN_STATE = HD + 4;      // floats of a column's state: O [HD], m, l, mo, one unused
+void launch_pattn_many(cudaStream_t s, const PagesAttn& a, int few, const CUtensorMap& tk, const CUtensorMap& tv);
 int pattn_few_status();
+int pattn_many_status();
 void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks, int most_cols);
 
 bool pattn_map(CUtensorMap* tm, const NslPages& p, const int8_t* codes);      // rows of hd codes, boxes of min(page, 64) rows, swizzled
@@ -47,16 +50,16 @@ __device__ __forceinline__ bool pa_bar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// Bounded: false after PATTN_WAIT_NS or PATTN_WAIT_LIMIT attempts, or once another warp of the block has given up.
+// By a whole warp.  Bounded: false after PATTN_WAIT_NS or PATTN_WAIT_LIMIT attempts, or once another warp of the block has given up.
 __device__ __forceinline__ bool pa_bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     unsigned long long t0 = 0;
     for (uint32_t i = 0; i < PATTN_WAIT_LIMIT; ++i) {
-        if (pa_bar_try(bar, parity)) return true;
+        if (__all_sync(0xFFFFFFFFu, pa_bar_try(bar, parity))) return true;
         if ((i & 63u) == 63u) {
             unsigned long long t;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
             if (!t0) t0 = t;
-            if (*abort_flag || t - t0 > PATTN_WAIT_NS) return false;
+            if (__any_sync(0xFFFFFFFFu, *abort_flag || t - t0 > PATTN_WAIT_NS)) return false;
         }
     }
     return false;

@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
             }
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const float by = pa_pow2_of(top), inv = 1.0f / by, fc = a.scale * 1.4426950408889634f * by;
+            const float by = pa_pow2_of(top), inv = copysignf(1.0f / by, a.scale), fc = fabsf(a.scale) * 1.4426950408889634f * by;
 #pragma unroll
             for (int j = 0; j < STEPS; ++j) {
                 qb[nt][j][0] = pa_f16x2(v[j][0] * inv, v[j][1] * inv);
@@ -405,9 +405,9 @@ static void launch_few(cudaStream_t s, const PagesAttn& a, int most, const CUten
 void launch_pattn_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
     const int group = a.n_head / a.p.n_kv;
     const bool narrow = (long long) group * a.max_rows <= 8;
-    if (a.p.hd == 128) { if (narrow) launch_few<128, 1>(s, a, 16, tk, tv); else launch_few<128, 2>(s, a, 16, tk, tv); }
-    else if (narrow) launch_few<64, 1>(s, a, 16, tk, tv);
-    else launch_few<64, 2>(s, a, 16, tk, tv);
+    if (a.p.hd == 128) { if (narrow) launch_few<128, 1>(s, a, PATTN_FEW, tk, tv); else launch_few<128, 2>(s, a, PATTN_FEW, tk, tv); }
+    else if (narrow) launch_few<64, 1>(s, a, PATTN_FEW, tk, tv);
+    else launch_few<64, 2>(s, a, PATTN_FEW, tk, tv);
 }
 
 }   // namespace nsl
