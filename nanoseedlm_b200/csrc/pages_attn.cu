@@ -119,9 +119,10 @@ void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, co
     a.part = (float*) ((char*) work + 16 * (size_t) pattn_blocks());
     a.scale = scale; a.q_type = q_type; a.q_stride = q_stride; a.o_type = o_type; a.o_stride = o_stride;
     a.n_head = n_head; a.layer = layer; a.window = window; a.n_seqs = n_seqs; a.max_rows = max_rows; a.T = T;
-    const int group = n_head / p->n_kv, few = group <= PATTN_FEW ? PATTN_FEW : 0;
-    if (few) launch_pattn_few(s, a, tk, tv);
-    if ((long long) group * (max_rows < T ? max_rows : T) > few) launch_pattn_many(s, a, few, tk, tv);
+    // One of the two for all sequences of a call: beside sequences of many rows those of few ones cost less in the wide kernel's blocks than
+    // in two more launches (32 decode rows of 4096 keys beside a chunk: see pages_attn_many.cu).
+    if ((long long) (n_head / p->n_kv) * (max_rows < T ? max_rows : T) <= PATTN_FEW) launch_pattn_few(s, a, tk, tv);
+    else launch_pattn_many(s, a, tk, tv);
 }
 
 }   // extern "C"

@@ -24,7 +24,7 @@ inline int pattn_blocks() { return 2 * sm_count(); }
 constexpr int PATTN_FEW = 16, PATTN_MANY = 256;      // columns of an item
 template <int HD>
 constexpr int PATTN_STATE = HD + 4;      // floats of a column's state: O [HD], m, l, mo, one unused
-void launch_pattn_many(cudaStream_t s, const PagesAttn& a, int few, const CUtensorMap& tk, const CUtensorMap& tv);
+void launch_pattn_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv);
 int pattn_few_status();
 int pattn_many_status();
 void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks, int most_cols);

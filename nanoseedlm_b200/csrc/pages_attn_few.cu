@@ -41,9 +41,9 @@ struct FewItem {      // a (sequence, KV head) and the units of it that a block 
 
 // Keys [k0, k1) that the rows of a descriptor attend, and its number of units per KV head (one at least: a row that attends
 // nothing is written too; 0 for descriptors without rows or with more columns than a tile holds).
-__device__ __forceinline__ int few_units(const PagesAttn& a, const RowSpan& sp, int group, int most, int* k0, int* k1) {
+__device__ __forceinline__ int few_units(const PagesAttn& a, const RowSpan& sp, int group, int* k0, int* k1) {
     *k0 = *k1 = 0;
-    if (sp.rows <= 0 || sp.rows * group > most) return 0;
+    if (sp.rows <= 0 || sp.rows * group > PATTN_FEW) return 0;
     const int last = sp.pos + sp.rows;
     *k1 = max(min(last, a.p.max_pages * a.p.page), 0);
     *k0 = a.window > 0 ? min(max(sp.pos - a.window + 1, 0), *k1) : 0;
@@ -53,11 +53,11 @@ __device__ __forceinline__ int few_units(const PagesAttn& a, const RowSpan& sp, 
 // The walk over a block's units: next() gives the item that unit x lies in.  Every warp keeps its own.
 struct FewWalk {
     int i, before;      // descriptor, units of the step before it
-    __device__ bool next(const PagesAttn& a, int group, int most, int x, int xe, FewItem* it) {
+    __device__ bool next(const PagesAttn& a, int group, int x, int xe, FewItem* it) {
         if (x >= xe) return false;
         for (; i < a.n_seqs; ++i) {
             it->sp = row_span(a, i);
-            const int n = few_units(a, it->sp, group, most, &it->k0, &it->k1);
+            const int n = few_units(a, it->sp, group, &it->k0, &it->k1);
             if (x < before + n * a.p.n_kv) {
                 it->kvh = (x - before) / n;
                 it->first = before + it->kvh * n;
@@ -117,7 +117,7 @@ __device__ __forceinline__ void few_weights(const float* p, int c, float* cw, fl
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, int most, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
+__global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
     using F = Few<HD, NT>;
     constexpr int CT = F::CT, STATE = F::STATE, STEPS = HD / 16;
     extern __shared__ uint8_t few_raw[];
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
     grid_dependency_wait();
     // the step's units, and the descriptor that this block's first lies in
     int total = 0, k0, k1;
-    for (int i = tid; i < a.n_seqs; i += FEW_THREADS) total += few_units(a, row_span(a, i), group, most, &k0, &k1) * a.p.n_kv;
+    for (int i = tid; i < a.n_seqs; i += FEW_THREADS) total += few_units(a, row_span(a, i), group, &k0, &k1) * a.p.n_kv;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
     if (lane == 0) wsum[warp] = total;
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
     if (x0 >= xe) return;
     if (tid == 0) { plan[0] = 0; plan[1] = 0; }
     for (int base = 0, before = 0; base < a.n_seqs; base += FEW_THREADS) {
-        const int i = base + tid, mine = i < a.n_seqs ? few_units(a, row_span(a, i), group, most, &k0, &k1) * a.p.n_kv : 0;
+        const int i = base + tid, mine = i < a.n_seqs ? few_units(a, row_span(a, i), group, &k0, &k1) * a.p.n_kv : 0;
         int incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o); if (lane >= o) incl += v; }
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
         const int batch = 32 / pieces;      // units a look ahead covers
         int x = x0;
         bool ok = true;
-        while (ok && walk.next(a, group, most, x, xe, &it)) {
+        while (ok && walk.next(a, group, x, xe, &it)) {
             const size_t head_at = (size_t) a.layer * a.p.n_pages * a.p.n_kv + it.kvh;
             for (int b = it.x0; ok && b < it.x1; b += batch) {
                 // lane j: piece j from position p on
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
     const uint32_t l_at = (uint32_t) (16 * warp + lrow) * HD, l_x = (uint32_t) (lane >> 4) ^ sw;
     float* const merge = (float*) (smem + F::OFF_MERGE);
     int x = x0;
-    while (walk.next(a, group, most, x, xe, &it)) {
+    while (walk.next(a, group, x, xe, &it)) {
         const int cols = it.sp.rows * group;
         // the queries as B fragments: column r0 of a tile, dims 16 j + 4 q4 ..; a column divided by its power of two
         uint32_t qb[NT][STEPS][2];
@@ -394,20 +394,20 @@ int pattn_few_status() {
 }
 
 template <int HD, int NT>
-static void launch_few(cudaStream_t s, const PagesAttn& a, int most, const CUtensorMap& tk, const CUtensorMap& tv) {
+static void launch_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
     cudaFuncSetAttribute(pattn_few_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<HD, NT>::SMEM);
-    launch(pattn_few_kernel<HD, NT>, (unsigned) pattn_blocks(), FEW_THREADS, Few<HD, NT>::SMEM, s, a, most, tk, tv);
+    launch(pattn_few_kernel<HD, NT>, (unsigned) pattn_blocks(), FEW_THREADS, Few<HD, NT>::SMEM, s, a, tk, tv);
     launch_pattn_merge(s, a, pattn_blocks(), Few<HD, NT>::CT);
     count_launch(2);
 }
 
-// Sequences of at most 16 columns; the others are passed over.
+// Sequences of at most PATTN_FEW columns.
 void launch_pattn_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
     const int group = a.n_head / a.p.n_kv;
     const bool narrow = (long long) group * a.max_rows <= 8;
-    if (a.p.hd == 128) { if (narrow) launch_few<128, 1>(s, a, PATTN_FEW, tk, tv); else launch_few<128, 2>(s, a, PATTN_FEW, tk, tv); }
-    else if (narrow) launch_few<64, 1>(s, a, PATTN_FEW, tk, tv);
-    else launch_few<64, 2>(s, a, PATTN_FEW, tk, tv);
+    if (a.p.hd == 128) { if (narrow) launch_few<128, 1>(s, a, tk, tv); else launch_few<128, 2>(s, a, tk, tv); }
+    else if (narrow) launch_few<64, 1>(s, a, tk, tv);
+    else launch_few<64, 2>(s, a, tk, tv);
 }
 
 }   // namespace nsl

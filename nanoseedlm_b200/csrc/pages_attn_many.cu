@@ -2,23 +2,27 @@
 //
 // An item is 256 columns ((row, query head) pairs of a KV head) of a sequence as two tiles of 128; a unit is 64 keys of an item.
 // The step's units are dealt evenly to the blocks, one an SM, in order; a run that ends inside an item leaves its state for the
-// merge kernel.  Per unit, on both tiles:
-//   S [128][64]  = Q [128][hd] . K^T      A = queries (f16, tensor memory), B = keys [64][hd] in shared memory
-//   O [128][hd] += W [128][64] . V        A = weights (f16, over S in tensor memory), B = values as [hd][64] in shared memory
+// merge kernel.  Per unit and tile:
+//   S [128][64]  = Q [128][hd] . K^T      A = queries (f16; the first tile's in tensor memory, the second's in shared memory), B = keys [64][hd]
+//   O [128][hd] += W [128][64] . V        A = weights (f16, tensor memory), B = values as [hd][64]
 // Warps: 4 + 4 take the softmax of the two tiles (a thread a column: its row of S is in its tensor memory lane), 4 expand the
-// codes to f16 (exact) into the layout the products read, 1 fetches pages, 1 issues the products.  While one tile's scores are
-// in its softmax, the other's products run.  The two scales and the running maxima are as in pages_attn_few.cu; here the maxima
-// that the exponents use follow the true ones only when these have grown by 2^8 (weights up to 2^8 then), so O in tensor memory
-// is hardly ever rescaled.
-// Bound: the exponentials (16 a clock and SM: 128 x 64 x 2 a unit take 1024 clk) and the products (1024 clk) alike.
+// codes to f16 (exact) into the layout the products read, 1 fetches pages, 1 issues the products: the scores of a tile's next
+// unit as soon as the last ones are in registers, the values once the weights are there.  An item of up to 128 columns has both
+// tiles work on the same queries, every other unit each, and their states joined at its end.
+// The two scales and the running maxima are as in pages_attn_few.cu; here the maxima that the exponents use follow the true ones
+// only when these have grown by 2^8 (weights up to 2^8 then), so O in tensor memory is hardly ever rescaled.
+// Bound: a unit of two tiles takes 1024 clk of exponentials (16 a clock and SM), 1024 clk of products, about 1300 clk of shared
+// memory (codes in, f16 out, and what the products read) and 1000 issue slots a scheduler.
+#include <type_traits>
+
 #include "pages_attn.cuh"
 #include "seed_block.cuh"
 
 namespace nsl {
 
-constexpr int MANY_KEYS = 64, MANY_TILE = 128, MANY_COLS = PATTN_MANY, MANY_THREADS = 448, MANY_RAW = 4, MANY_STAGES = 4, MANY_META = 16;
+constexpr int MANY_KEYS = 64, MANY_TILE = 128, MANY_COLS = PATTN_MANY, MANY_THREADS = 448, MANY_RAW = 3, MANY_STAGES = 4, MANY_META = 16;
 constexpr int MANY_EXPAND = 8, MANY_FETCH = 12, MANY_MMA = 13;      // first warp of each part; the softmax has warps 0 .. 7
-constexpr int TM_S = 0, TM_Q = 128, TM_O = 256;                      // tensor memory columns: S (64 a tile; W is its first 32), Q (64 a tile), O (128 a tile)
+constexpr int TM_S = 0, TM_Q = 128, TM_W = 192, TM_O = 256;         // tensor memory columns: S (64 a tile), the first tile's Q (64), W (32 a tile), O (128 a tile)
 constexpr float MANY_SLACK = 8.0f;                                   // how far (in powers of 2) a weight may exceed 1
 
 template <int HD>
@@ -26,12 +30,14 @@ struct Many {
     static constexpr int RAW = MANY_KEYS * HD;                       // bytes of a unit's key codes, or value codes
     static constexpr int TILE = 2 * RAW;                             // the same as f16
     static constexpr int OFF_TILES = MANY_RAW * 2 * RAW;
-    static constexpr int OFF_META = OFF_TILES + MANY_STAGES * 2 * TILE;
+    static constexpr int OFF_Q = OFF_TILES + MANY_STAGES * 2 * TILE; // the second tile's queries
+    static constexpr int OFF_META = OFF_Q + 2 * MANY_TILE * HD;
     static constexpr int OFF_BARS = OFF_META + MANY_META * 4 * 16;
-    static constexpr int BARS = 2 * MANY_RAW + 2 * MANY_STAGES + MANY_META + 9;
+    static constexpr int BARS = 2 * MANY_RAW + 2 * MANY_STAGES + MANY_META + 11;
     static constexpr int SMEM = OFF_BARS + 8 * BARS + 1024;
 };
 static_assert(MANY_COLS == 2 * MANY_TILE, "two tiles an item");
+static_assert(Many<128>::SMEM + 2048 <= 232448, "shared memory");
 constexpr int MANY_SEQS = 4096;      // descriptors of a call; their units sit in the tiles' memory while the plan is made
 static_assert(MANY_SEQS * 4 <= MANY_STAGES * 4 * 64 * 64, "the plan's memory");
 
@@ -50,8 +56,6 @@ __device__ __forceinline__ int many_units(const PagesAttn& a, const RowSpan& sp,
     *k0 = a.window > 0 ? min(max(sp.pos + i0 - a.window + 1, 0), *k1) : 0;
     return max((*k1 + MANY_KEYS - 1) / MANY_KEYS - *k0 / MANY_KEYS, 1);
 }
-// Columns of a sequence, 0 for those that pages_attn_few.cu takes.
-__device__ __forceinline__ int many_cols(const RowSpan& sp, int group, int few) { return sp.rows * group > few ? sp.rows * group : 0; }
 __device__ __forceinline__ int warp_sum(int v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
@@ -61,12 +65,12 @@ __device__ __forceinline__ int warp_sum(int v) {
 // The walk over a block's units, by whole warps.
 struct ManyWalk {
     int i, before;
-    __device__ bool next(const PagesAttn& a, int group, int few, int x, int xe, ManyItem* it) {
+    __device__ bool next(const PagesAttn& a, int group, int x, int xe, ManyItem* it) {
         const int lane = threadIdx.x & 31;
         if (x >= xe) return false;
         for (; i < a.n_seqs; ++i) {
             it->sp = row_span(a, i);
-            const int cols = many_cols(it->sp, group, few), tiles = (cols + MANY_COLS - 1) / MANY_COLS;
+            const int cols = it->sp.rows * group, tiles = (cols + MANY_COLS - 1) / MANY_COLS;
             int at = before;      // units before the tiles looked at
             for (int t0 = 0; t0 < tiles; t0 += 32) {
                 int k0 = 0, k1 = 0;
@@ -103,12 +107,20 @@ __device__ __forceinline__ uint64_t many_desc(uint32_t saddr) {      // K-major,
 __device__ __forceinline__ constexpr uint32_t many_idesc(int n) {      // D f32, A and B f16, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
     return (1u << 4) | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (MANY_TILE >> 4) << 24);
 }
-__device__ __forceinline__ void many_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+// Called by the whole warp, issued by one elected lane: with operands that the warp shares the issue costs a few clocks, inside a branch
+// of one lane 60 (128 x 64 x 128 and 128 x 128 x 64 take 514 clk instead of 803).
+__device__ __forceinline__ void many_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {      // A in tensor memory
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t) add) : "memory");
 }
+__device__ __forceinline__ void many_mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {      // A in shared memory
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t) add) : "memory");
+}
+// x, the same in all lanes, as a value that the compiler knows to be so.
+__device__ __forceinline__ uint32_t same(uint32_t x) { return __reduce_or_sync(0xFFFFFFFFu, x); }
 __device__ __forceinline__ void many_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -119,12 +131,29 @@ __device__ __forceinline__ void tm_ld32(uint32_t at, uint32_t* v) {      // not 
                    "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
                  : "r"(at) : "memory");
 }
+__device__ __forceinline__ void tm_wait_ld();
+__device__ __forceinline__ void tm_ld16(uint32_t at, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+                   "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(at) : "memory");
+    tm_wait_ld();
+}
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+__device__ __forceinline__ void tm_st16(uint32_t at, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
-                   "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-                   "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+                   "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ bool softmax_sync(bool x) {      // the softmax warps of both tiles; whether any thread's x is true
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((uint32_t) x) : "memory");
+    return r != 0;
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void many_ldsm_trans(uint32_t* r, uint32_t at) {
@@ -142,26 +171,29 @@ __device__ __forceinline__ void many_sts(uint32_t at, uint32_t a, uint32_t b, ui
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-template <int HD>
-__global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a, int few, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
+// WIDE: pages of 64 and more positions, a unit's keys have one pair of scales.
+template <int HD, bool WIDE>
+__global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
     using F = Many<HD>;
-    constexpr int STATE = PATTN_STATE<HD>, WARPS = MANY_THREADS / 32;
+    constexpr int STATE = PATTN_STATE<HD>, WARPS = MANY_THREADS / 32, NG = WIDE ? 1 : 4, GK = MANY_KEYS / NG;      // groups of GK keys with one pair of scales
     extern __shared__ uint8_t many_raw[];
     uint8_t* const smem = (uint8_t*) (((uintptr_t) many_raw + 1023) & ~(uintptr_t) 1023);
     __shared__ int wsum[WARPS], plan[2], abort_flag;
     __shared__ uint32_t tmem_slot;
+    __shared__ float other[3][MANY_TILE];      // the second tile's m, l, mo where both have the same columns
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.n_head / a.p.n_kv;
     const uint32_t base = pa_smem(smem), tiles = base + F::OFF_TILES, bars = base + F::OFF_BARS;
-    // arrivals: raw_full the fetch (and bytes), raw_empty the 4 expanding warps, tile_full the same, tile_empty the products, meta the
-    // fetch; per tile: s_full the products, w_full the tile's 4 warps, q_full the same, o_full the products; done the products
+    // arrivals: raw_full the fetch (and bytes), raw_empty the 4 expanding warps, tile_full the same, tile_empty the products, meta the fetch;
+    // per tile: s_full and o_done (a unit's scores are there, its values are in O) the products, s_free (the scores are in registers),
+    // w_full and q_full the tile's 4 warps; done the products
     const uint32_t raw_full = bars, raw_empty = raw_full + 8 * MANY_RAW, tile_full = raw_empty + 8 * MANY_RAW, tile_empty = tile_full + 8 * MANY_STAGES, meta_full = tile_empty + 8 * MANY_STAGES,
-                   s_full = meta_full + 8 * MANY_META, w_full = s_full + 16, q_full = w_full + 16, o_full = q_full + 16, done = o_full + 16;
+                   s_full = meta_full + 8 * MANY_META, s_free = s_full + 16, w_full = s_free + 16, q_full = w_full + 16, o_done = q_full + 16, done = o_done + 16;
     const float4* const meta = (const float4*) (smem + F::OFF_META);
     if (tid == 0) {
         for (int i = 0; i < MANY_RAW; ++i) { pa_bar_init(raw_full + 8 * i, 1); pa_bar_init(raw_empty + 8 * i, 4); }
         for (int i = 0; i < MANY_STAGES; ++i) { pa_bar_init(tile_full + 8 * i, 4); pa_bar_init(tile_empty + 8 * i, 1); }
         for (int i = 0; i < MANY_META; ++i) pa_bar_init(meta_full + 8 * i, 1);
-        for (int t = 0; t < 2; ++t) { pa_bar_init(s_full + 8 * t, 1); pa_bar_init(w_full + 8 * t, 4); pa_bar_init(q_full + 8 * t, 4); pa_bar_init(o_full + 8 * t, 1); }
+        for (int t = 0; t < 2; ++t) { pa_bar_init(s_full + 8 * t, 1); pa_bar_init(s_free + 8 * t, 4); pa_bar_init(w_full + 8 * t, 4); pa_bar_init(q_full + 8 * t, 4); pa_bar_init(o_done + 8 * t, 1); }
         pa_bar_init(done, 1);
         abort_flag = 0;
         plan[0] = plan[1] = 0;
@@ -178,7 +210,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
     int total = 0;
     for (int i = warp; i < a.n_seqs; i += WARPS) {
         const RowSpan sp = row_span(a, i);
-        const int cols = many_cols(sp, group, few), nt = (cols + MANY_COLS - 1) / MANY_COLS;
+        const int cols = sp.rows * group, nt = (cols + MANY_COLS - 1) / MANY_COLS;
         int n = 0, k0, k1;
         for (int t = lane; t < nt; t += 32) n += many_units(a, sp, group, cols, t, &k0, &k1);
         n = warp_sum(n) * a.p.n_kv;
@@ -194,7 +226,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
     for (int w = 0; w < WARPS; ++w) total += wsum[w];
     const int per = max((total + (int) gridDim.x - 1) / (int) gridDim.x, 1);
     const int x0 = (int) blockIdx.x * per, xe = min(total, x0 + per);
-    const uint32_t tmem = tmem_slot;
+    constexpr uint32_t tmem = 0;      // all 512 columns are the block's
     if (tid == 0) a.rec[blockIdx.x] = make_int4(0, 0, 0, 0);      // (thread 0 writes it again below)
     for (int from = 0, before = 0; from < a.n_seqs; from += MANY_THREADS) {
         const int mine = from + tid < a.n_seqs ? of_seq[from + tid] : 0;
@@ -215,23 +247,22 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
     ManyWalk walk = {plan[0], plan[1]};
     ManyItem it;
     volatile int* const ab = &abort_flag;
-    bool ok = true;
+    bool ok = tmem_slot == tmem;      // (it is: nothing else can have been allocated)
     auto fail = [&](int code) { abort_flag = 1; atomicCAS(&g_pattn_many_status, 0, code); ok = false; };
     int g = 0;      // units this block has done: the rings' position
 
     if (warp < MANY_EXPAND) {      // ---- softmax: tile t, column c of it ----
         const int t = warp >> 2, c = 32 * (warp & 3) + lane;
-        const uint32_t lanes = tmem + ((uint32_t) (32 * (warp & 3)) << 16), ts = lanes + TM_S + 64 * t, tq = lanes + TM_Q + 64 * t, to = lanes + TM_O + 128 * t;
-        int items = 0, steps = 0;      // of this tile: phases of its barriers
-        for (int x = x0; ok && walk.next(a, group, few, x, xe, &it); x = it.x1) {
-            const int n = it.x1 - it.x0, col = it.col0 + MANY_TILE * t + c;
-            if (it.cols <= MANY_TILE * t) { g += n; continue; }      // the tile is empty
-            const bool valid = MANY_TILE * t + c < it.cols, warp_valid = MANY_TILE * t + 32 * (warp & 3) < it.cols;
+        const uint32_t lanes = tmem + ((uint32_t) (32 * (warp & 3)) << 16), ts = lanes + TM_S + 64 * t, tw = lanes + TM_W + 32 * t, to = lanes + TM_O + 128 * t;
+        int steps = 0;      // of this tile: phases of its barriers
+        for (int x = x0; walk.next(a, group, x, xe, &it); x = it.x1) {
+            // up to 128 columns: both tiles have them, and every other unit each
+            const int shared = it.cols <= MANY_TILE, n = shared ? (it.x1 - it.x0 + 1 - t) / 2 : it.x1 - it.x0, c0 = shared ? 0 : MANY_TILE * t, col = it.col0 + c0 + c;
+            const bool valid = c0 + c < it.cols, warp_valid = c0 + 32 * (warp & 3) < it.cols;
             const int row = it.sp.row + col / group, head = it.kvh * group + col % group, pos = it.sp.pos + col / group;
             const int hi = valid ? pos : -1, lo = valid && a.window > 0 ? pos - a.window + 1 : 0;
             float f = 0.0f;      // scale, log2 e and the power of two that the query is divided by
             if (warp_valid) {
-                // where no key of a unit is masked for any column of the warp
                 float top = 0.0f;
                 const size_t at = (size_t) row * a.q_stride + (size_t) head * HD;
                 if (valid)
@@ -245,10 +276,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                 const float by = pa_pow2_of(top), inv = copysignf(1.0f / by, a.scale);      // the scale's sign goes with the query: maxima are then of scores
                 f = fabsf(a.scale) * 1.4426950408889634f * by;
 #pragma unroll
-                for (int d = 0; d < HD; d += 64) {
-                    uint32_t w[32];
+                for (int d = 0; d < HD; d += 32) {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < 4; ++j) {
                         float v[8];
                         if (!valid) {
 #pragma unroll
@@ -257,10 +288,14 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                         else load8<NSL_F32>(a.q, at + d + 8 * j, v);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) w[4 * j + e] = pa_f16x2(v[2 * e] * inv, v[2 * e + 1] * inv);
+                        if (t == 1)      // panels of 64 dims, rows of 128 bytes
+                            many_sts(base + F::OFF_Q + (d >> 6) * (MANY_TILE * 128) + c * 128 + (((uint32_t) ((d & 63) / 8 + j) ^ (uint32_t) (c & 7)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2],
+                                     w[4 * j + 3]);
                     }
-                    tm_st32(tq + d / 2, w);
+                    if (t == 0) tm_st16(lanes + TM_Q + d / 2, w);
                 }
-                tm_wait_st();
+                if (t == 0) tm_wait_st();
+                else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
             tm_before();
             __syncwarp();
@@ -269,115 +304,175 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
             const int all_hi = __shfl_sync(0xFFFFFFFFu, pos, 0);
             const int all_lo = a.window > 0 ? __reduce_max_sync(0xFFFFFFFFu, valid ? lo : -2147483647 - 1) : 0;
             float m = -INFINITY, mo = -INFINITY, l = 0.0f;
-            for (int j = 0; j < n; ++j, ++g, ++steps) {
-                if (!pa_bar_wait(s_full + 8 * t, steps & 1, ab) || !pa_bar_wait(meta_full + 8 * (g % MANY_META), g / MANY_META & 1, ab)) { fail(4); break; }
+            for (int j = 0; j < n; ++j, ++steps) {
+                const int u = shared ? 2 * j + t : j, at = g + u;      // the unit; its place in the rings
+                if (!pa_bar_wait(s_full + 8 * t, steps & 1, ab) || !pa_bar_wait(meta_full + 8 * (at % MANY_META), at / MANY_META & 1, ab)) { fail(4); break; }
                 tm_after();
-                if (warp_valid) {
-                    uint32_t su[64];
-                    float* const s = (float*) su;
-                    tm_ld32(ts, su);
-                    tm_ld32(ts + 32, su + 32);
-                    float4 mt[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) mt[i] = meta[4 * (g % MANY_META) + i];
-                    const int key = (it.tile0 + it.x0 + j - it.first) * MANY_KEYS;
-                    tm_wait_ld();
-                    float fg[4];      // scores = s * fg
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) fg[i] = f * mt[i].x;
-                    if (key + MANY_KEYS - 1 > all_hi || key < all_lo || mt[0].z + mt[1].z + mt[2].z + mt[3].z != 4.0f) {
-#pragma unroll
-                        for (int i = 0; i < 64; ++i) {
-                            const bool seen = key + i <= hi && key + i >= lo && mt[i >> 4].z != 0.0f;
-                            s[i] = seen ? s[i] * fg[i >> 4] : -INFINITY;
-                        }
-                        fg[0] = fg[1] = fg[2] = fg[3] = 1.0f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) if (mt[i].z == 0.0f) mt[i].y = 0.0f;
-                    }
-                    float mx[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        mx[i] = s[16 * i];
-#pragma unroll
-                        for (int e = 1; e < 16; ++e) mx[i] = fmaxf(mx[i], s[16 * i + e]);
-                        mx[i] *= fg[i];
-                    }
-                    const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), mon = fmaxf(fmaxf(mx[0] + mt[0].y, mx[1] + mt[1].y), fmaxf(mx[2] + mt[2].y, mx[3] + mt[3].y));
-                    if (mn > m + MANY_SLACK || (m == -INFINITY && mn > m)) { l *= pa_ex2(m - mn); m = mn; }
-                    const bool up = mon > mo + MANY_SLACK || (mo == -INFINITY && mon > mo);
-                    if (__any_sync(0xFFFFFFFFu, up)) {
-                        const float cor = up ? pa_ex2(mo - mon) : 1.0f;
-                        if (up) mo = mon;
-                        if (j > 0)      // (the product before this unit's has ended: its scores came behind it)
-#pragma unroll 1
-                            for (int d = 0; d < HD; d += 32) {
-                                uint32_t v[32];
-                                tm_ld32(to + d, v);
-                                tm_wait_ld();
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * cor);
-                                tm_st32(to + d, v);
-                            }
-                    }
-                    const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
-                    uint32_t w[32];
-                    u64 sum = pack2(0.0f, 0.0f);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float cf = pa_ex2(fminf(mt[i].y + (ms - mos), 120.0f));      // weight = p cf (finite: a weight whose p is 0 is 0)
-                        const u64 f2 = pack2(fg[i], fg[i]), m2 = pack2(-ms, -ms), c2 = pack2(cf, cf);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            float p0, p1;
-                            unpack2(fma2(pack2(s[16 * i + 2 * e], s[16 * i + 2 * e + 1]), f2, m2), p0, p1);
-                            const u64 p = pack2(pa_ex2(p0), pa_ex2(p1));
-                            sum = add2(sum, p);
-                            float w0, w1;
-                            unpack2(mul2(p, c2), w0, w1);
-                            w[8 * i + e] = pa_f16x2(w0, w1);
-                        }
-                    }
-                    float l0, l1;
-                    unpack2(sum, l0, l1);
-                    l += l0 + l1;
-                    tm_st32(ts, w);
-                    tm_wait_st();
+                if (!warp_valid) {
+                    __syncwarp();
+                    if (lane == 0) { pa_bar_arrive(s_free + 8 * t); pa_bar_arrive(w_full + 8 * t); }
+                    continue;
                 }
+                uint32_t su[64];
+                float* const s = (float*) su;
+                tm_ld32(ts, su);
+                tm_ld32(ts + 32, su + 32);
+                float fg[NG], lv[NG];      // scores = s * fg; log2 of the value scales
+                bool whole = true;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const float4 mt = meta[4 * (at % MANY_META) + i];
+                    fg[i] = f * mt.x;
+                    lv[i] = mt.y;
+                    whole = whole && mt.z != 0.0f;
+                }
+                const int key = (it.tile0 + it.x0 + u - it.first) * MANY_KEYS;
+                tm_wait_ld();
+                tm_before();
+                __syncwarp();
+                if (lane == 0) pa_bar_arrive(s_free + 8 * t);
+                if (key + MANY_KEYS - 1 > all_hi || key < all_lo || !whole) {
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        const bool there = meta[4 * (at % MANY_META) + i].z != 0.0f;
+#pragma unroll
+                        for (int e = GK * i; e < GK * i + GK; ++e) s[e] = there && key + e <= hi && key + e >= lo ? s[e] * fg[i] : -INFINITY;
+                        fg[i] = 1.0f;
+                        if (!there) lv[i] = 0.0f;
+                    }
+                }
+                float mn = -INFINITY, mon = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    float a0 = max3(s[GK * i], s[GK * i + 1], s[GK * i + 2]), a1 = s[GK * i + 3];
+#pragma unroll
+                    for (int e = 4; e < GK; e += 4) { a0 = max3(a0, s[GK * i + e], s[GK * i + e + 1]); a1 = max3(a1, s[GK * i + e + 2], s[GK * i + e + 3]); }
+                    const float mx = fmaxf(a0, a1) * fg[i];
+                    mn = fmaxf(mn, mx);
+                    mon = fmaxf(mon, mx + lv[i]);
+                }
+                if (mn > m + MANY_SLACK || (m == -INFINITY && mn > m)) { l *= pa_ex2(m - mn); m = mn; }
+                const bool up = mon > mo + MANY_SLACK || (mo == -INFINITY && mon > mo);
+                const bool any_up = __any_sync(0xFFFFFFFFu, up);
+                // the tile's last values are in O, and its last weights have been read
+                if (j > 0 && !pa_bar_wait(o_done + 8 * t, (steps - 1) & 1, ab)) { fail(5); break; }
+                if (any_up) {
+                    const float cor = up ? pa_ex2(mo - mon) : 1.0f;
+                    if (up) mo = mon;
+                    if (j > 0) {
+                        tm_after();
+#pragma unroll 1
+                        for (int d = 0; d < HD; d += 16) {
+                            uint32_t v[16];
+                            tm_ld16(to + d, v);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * cor);
+                            tm_st16(to + d, v);
+                        }
+                    }
+                }
+                const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
+                // a weight is p cf, p = 2^(score - m), cf = 2^lc: one exponential of the sum, p's sum from the weights' sum, unless
+                // the two lie so far apart that a weight underflows where its p counts
+                float lc[NG];
+                bool near = true;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) { lc[i] = lv[i] + (ms - mos); near = near && fabsf(lc[i]) <= 64.0f; }
+                if (__all_sync(0xFFFFFFFFu, near)) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = WIDE ? 0 : 2 * h; i < (WIDE ? 1 : 2 * h + 2); ++i) {
+                            const u64 f2 = pack2(fg[i], fg[i]), b2 = pack2(lc[i] - ms, lc[i] - ms);
+                            u64 sum = pack2(0.0f, 0.0f);
+                            constexpr int PAIRS = WIDE ? 16 : 8;
+                            const int e0 = WIDE ? 32 * h : 16 * i;
+#pragma unroll
+                            for (int e = 0; e < PAIRS; ++e) {
+                                float w0, w1;
+                                unpack2(fma2(pack2(s[e0 + 2 * e], s[e0 + 2 * e + 1]), f2, b2), w0, w1);
+                                w0 = pa_ex2(w0); w1 = pa_ex2(w1);
+                                sum = add2(sum, pack2(w0, w1));
+                                w[e0 / 2 - 16 * h + e] = pa_f16x2(w0, w1);
+                            }
+                            float l0, l1;
+                            unpack2(sum, l0, l1);
+                            l = fmaf(l0 + l1, pa_ex2(-lc[i]), l);
+                        }
+                        tm_st16(tw + 16 * h, w);
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int k = 32 * h + 2 * e, i = k / GK;
+                            const float cf = pa_ex2(fminf(lc[i], 120.0f));      // finite: a weight whose p is 0 is 0
+                            const float p0 = pa_ex2(fmaf(s[k], fg[i], -ms)), p1 = pa_ex2(fmaf(s[k + 1], fg[i], -ms));
+                            l += p0 + p1;
+                            w[e] = pa_f16x2(p0 * cf, p1 * cf);
+                        }
+                        tm_st16(tw + 16 * h, w);
+                    }
+                }
+                tm_wait_st();
                 tm_before();
                 __syncwarp();
                 if (lane == 0) pa_bar_arrive(w_full + 8 * t);
             }
-            if (!ok) break;
+            if (ok && n > 0 && !pa_bar_wait(o_done + 8 * t, (steps - 1) & 1, ab)) fail(5);
             // ---- results ----
-            if (!pa_bar_wait(o_full + 8 * t, items & 1, ab)) { fail(5); break; }
-            ++items;
-            tm_after();
             const int b0 = it.first / per, parts = (it.first + it.units - 1) / per - b0 + 1;
-            if (warp_valid) {
-                const float by = parts == 1 ? pattn_factor(m, l, mo) : 1.0f;
-                float* const part = a.part + ((size_t) (2 * blockIdx.x + ((int) blockIdx.x == b0)) * MANY_COLS + MANY_TILE * t + c) * STATE;
+            float by = 1.0f, by1 = 0.0f;      // what this tile's and the second's O are multiplied with
+            if (shared && t == 1) { other[0][c] = m; other[1][c] = l; other[2][c] = mo; }
+            tm_before();
+            if (softmax_sync(!ok)) { ok = false; break; }      // (all eight warps stay together, whatever fails)
+            tm_after();
+            if (shared) {
+                if (t == 0) {
+                    const float m1 = other[0][c], mo1 = other[2][c], mm = fmaxf(m, m1), mmo = fmaxf(mo, mo1);
+                    const float ms = mm == -INFINITY ? 0.0f : mm, mos = mmo == -INFINITY ? 0.0f : mmo;
+                    l = l * pa_ex2(m - ms) + other[1][c] * pa_ex2(m1 - ms);
+                    by = pa_ex2(mo - mos);
+                    by1 = pa_ex2(mo1 - mos);
+                    m = mm;
+                    mo = mmo;
+                }
+            }
+            if (warp_valid && !(shared && t)) {
+                const float fac = parts == 1 ? pattn_factor(m, l, mo) : 1.0f;
+                const bool first = it.x1 - it.x0 > 0, second = shared && it.x1 - it.x0 > 1;      // (an O that nothing was added to holds anything)
+                float* const part = a.part + ((size_t) (2 * blockIdx.x + ((int) blockIdx.x == b0)) * MANY_COLS + c0 + c) * STATE;
                 const size_t at = (size_t) row * a.o_stride + (size_t) head * HD;
 #pragma unroll 1
-                for (int d = 0; d < HD; d += 32) {
-                    uint32_t v[32];
-                    tm_ld32(to + d, v);
-                    tm_wait_ld();
+                for (int d = 0; d < HD; d += 16) {
+                    uint32_t v[16], v1[16];
+                    tm_ld16(to + d, v);
+                    if (second) tm_ld16(to + 128 + d, v1);
                     if (!valid) continue;
                     // product row n = 16 j + r: dim 16 j + 2 r, n = 16 j + 8 + r: the next
+                    float o[16];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float o[16];
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) { o[2 * r] = __uint_as_float(v[16 * j + r]) * by; o[2 * r + 1] = __uint_as_float(v[16 * j + 8 + r]) * by; }
-                        if (parts > 1) { store8<NSL_F32>(part, d + 16 * j, o); store8<NSL_F32>(part, d + 16 * j + 8, o + 8); }
-                        else if (a.o_type == NSL_BF16) { store8<NSL_BF16>(a.o, at + d + 16 * j, o); store8<NSL_BF16>(a.o, at + d + 16 * j + 8, o + 8); }
-                        else { store8<NSL_F32_BF16>(a.o, at + d + 16 * j, o); store8<NSL_F32_BF16>(a.o, at + d + 16 * j + 8, o + 8); }
+                    for (int r = 0; r < 16; ++r) {
+                        float z = first ? __uint_as_float(v[r]) * by : 0.0f;
+                        if (second) z = fmaf(__uint_as_float(v1[r]), by1, z);
+                        o[r < 8 ? 2 * r : 2 * (r - 8) + 1] = z * fac;
                     }
+                    if (parts > 1) { store8<NSL_F32>(part, d, o); store8<NSL_F32>(part, d + 8, o + 8); }
+                    else if (a.o_type == NSL_BF16) { store8<NSL_BF16>(a.o, at + d, o); store8<NSL_BF16>(a.o, at + d + 8, o + 8); }
+                    else { store8<NSL_F32_BF16>(a.o, at + d, o); store8<NSL_F32_BF16>(a.o, at + d + 8, o + 8); }
                 }
                 if (parts > 1 && valid) *(float4*) (part + HD) = make_float4(m, l, mo, 0.0f);
             }
+            if (shared) {      // the second tile's O has been read
+                tm_before();
+                softmax_sync(false);
+                tm_after();
+            }
             if (tid == 0 && parts > 1 && (int) blockIdx.x == b0) a.rec[blockIdx.x] = make_int4(parts | it.kvh << 16, it.sp.row, it.col0, it.cols);
+            g += it.x1 - it.x0;
         }
     } else if (warp < MANY_FETCH) {      // ---- expands codes ----
         const int w = warp - MANY_EXPAND, e = tid - 32 * MANY_EXPAND;
@@ -428,7 +523,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
         asm volatile("fence.proxy.async;" ::: "memory");      // codes that the kernel before has stored
         const int piece = min(a.p.page, MANY_KEYS), pieces = MANY_KEYS / piece, batch = 32 / pieces;
         float4* const meta_to = (float4*) (smem + F::OFF_META);
-        for (int x = x0; ok && walk.next(a, group, few, x, xe, &it); x = it.x1) {
+        for (int x = x0; ok && walk.next(a, group, x, xe, &it); x = it.x1) {
             const size_t head_at = (size_t) a.layer * a.p.n_pages * a.p.n_kv + it.kvh;
             for (int b = it.x0; ok && b < it.x1; b += batch) {
                 const int p = (it.tile0 + b - it.first) * MANY_KEYS + lane * piece;      // lane j: piece j from here on
@@ -469,51 +564,57 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                 if (filled > 0) for (uint32_t k = 0; k < (1u << 20) && !pa_bar_try(raw_full + 8 * i, (filled - 1) & 1); ++k) {}
             }
     } else {      // ---- issues the products ----
-        const uint32_t id_s = many_idesc(MANY_KEYS), id_o = many_idesc(HD);
-        int items[2] = {0, 0}, steps[2] = {0, 0};
-        auto scores = [&](int t, int stage) {
-            const uint64_t kd = many_desc(tiles + stage * 2 * F::TILE);
+        // everything that an operand is made of comes from constants, counters and values that the warp is known to share (same())
+        constexpr uint32_t id_s = many_idesc(MANY_KEYS), id_o = many_idesc(HD);
+        const uint64_t qd = many_desc(base + F::OFF_Q), kd0 = many_desc(tiles), vd0 = many_desc(tiles + F::TILE);
+        uint32_t items = 0, units = 0, scored[2] = {0, 0}, summed[2] = {0, 0};      // of this block so far; of a tile: units scored, values added
+        for (int x = x0; ok && walk.next(a, group, x, xe, &it); x = it.x1, ++items) {
+            const uint32_t run = same(it.x1 - it.x0), shared = same(it.cols <= MANY_TILE), n = shared ? run : 2 * run;
+            if (!pa_bar_wait(q_full, items & 1, ab) || !pa_bar_wait(q_full + 8, items & 1, ab)) { fail(8); break; }
+            tm_after();
+            // step i: the scores of tile i & 1, then the values of its step before
+            auto step = [&](auto tile, uint32_t i) {
+                constexpr int t = decltype(tile)::value;
+                if (i < n) {
+                    const uint32_t at = units + (shared ? i : i >> 1), stage = at % MANY_STAGES;
+                    if (!pa_bar_wait(tile_full + 8 * stage, at / MANY_STAGES & 1, ab) || (scored[t] > 0 && !pa_bar_wait(s_free + 8 * t, (scored[t] - 1) & 1, ab))) { fail(9); return; }
+                    tm_after();
+                    ++scored[t];
+                    const uint64_t kd = kd0 + (uint64_t) (stage * (2 * F::TILE >> 4));
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) many_mma(tmem + TM_S + 64 * t, tmem + TM_Q + 64 * t + 8 * k, kd + (uint64_t) (((k >> 2) * (MANY_KEYS * 128) + (k & 3) * 32) >> 4), id_s, k > 0);
-            many_commit(s_full + 8 * t);
-        };
-        for (int x = x0; ok && walk.next(a, group, few, x, xe, &it); x = it.x1) {
-            const int n = it.x1 - it.x0, both = it.cols > MANY_TILE ? 2 : 1;
-            for (int t = 0; t < both; ++t)
-                if (!pa_bar_wait(q_full + 8 * t, items[t]++ & 1, ab)) { fail(8); break; }
-            for (int j = -1; ok && j < n; ++j) {      // unit j's values, unit j + 1's scores
-                for (int t = 0; t < both; ++t) {
-                    if (j >= 0) {
-                        if (!pa_bar_wait(w_full + 8 * t, steps[t]++ & 1, ab)) { fail(9); break; }
-                        tm_after();
-                        if (lane == 0) {
-                            const int stage = (g + j) % MANY_STAGES;
-                            const uint64_t vd = many_desc(tiles + stage * 2 * F::TILE + F::TILE);
-#pragma unroll
-                            for (int k = 0; k < MANY_KEYS / 16; ++k) many_mma(tmem + TM_O + 128 * t, tmem + TM_S + 64 * t + 8 * k, vd + (uint64_t) (2 * k), id_o, j > 0 || k > 0);
-                            if (j == n - 1) many_commit(o_full + 8 * t);
-                            if (t == both - 1) many_commit(tile_empty + 8 * stage);
-                        }
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const uint64_t kk = kd + (uint64_t) (((k >> 2) * (MANY_KEYS * 128) + (k & 3) * 32) >> 4);
+                        if (t == 0) many_mma(TM_S, TM_Q + 8 * k, kk, id_s, k > 0);
+                        else many_mma_smem(TM_S + 64, qd + (uint64_t) (((k >> 2) * (MANY_TILE * 128) + (k & 3) * 32) >> 4), kk, id_s, k > 0);
                     }
-                    if (j + 1 < n) {
-                        const int next = g + j + 1;
-                        if (t == 0 && !pa_bar_wait(tile_full + 8 * (next % MANY_STAGES), next / MANY_STAGES & 1, ab)) { fail(10); break; }
-                        tm_after();
-                        if (lane == 0) scores(t, next % MANY_STAGES);
-                    }
-                    __syncwarp();
+                    many_commit(s_full + 8 * t);
                 }
+                if (i >= 2 && i < n + 2) {
+                    const uint32_t at = units + (shared ? i - 2 : (i - 2) >> 1), stage = at % MANY_STAGES;
+                    if (!pa_bar_wait(w_full + 8 * t, summed[t] & 1, ab)) { fail(10); return; }
+                    tm_after();
+                    ++summed[t];
+                    const uint64_t vd = vd0 + (uint64_t) (stage * (2 * F::TILE >> 4));
+#pragma unroll
+                    for (int k = 0; k < MANY_KEYS / 16; ++k) many_mma(TM_O + 128 * t, TM_W + 32 * t + 8 * k, vd + (uint64_t) (2 * k), id_o, i >= 4 || k > 0);
+                    many_commit(o_done + 8 * t);
+                    if (shared || t == 1) many_commit(tile_empty + 8 * stage);
+                }
+            };
+            for (uint32_t i = 0; ok && i < n + 2; i += 2) {
+                step(std::integral_constant<int, 0>(), i);
+                if (ok) step(std::integral_constant<int, 1>(), i + 1);
             }
-            g += n;
+            units += run;
         }
-        if (lane == 0) many_commit(done);      // what has been issued ends before the tensor memory is given back
+        many_commit(done);      // what has been issued ends before the tensor memory is given back
         __syncwarp();
         for (uint32_t k = 0; k < (1u << 24) && !pa_bar_try(done, 0); ++k) {}
     }
     tm_before();
     __syncthreads();
     tm_after();
-    if (warp == MANY_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == MANY_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_slot) : "memory");
 }
 
 int pattn_many_status() {
@@ -523,18 +624,20 @@ int pattn_many_status() {
     return v;
 }
 
-// Sequences of more than `few` columns.
-void launch_pattn_many(cudaStream_t s, const PagesAttn& a, int few, const CUtensorMap& tk, const CUtensorMap& tv) {
+template <int HD, bool WIDE>
+static void launch_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
     const unsigned blocks = (unsigned) sm_count();
-    if (a.p.hd == 128) {
-        cudaFuncSetAttribute(pattn_many_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<128>::SMEM);
-        launch(pattn_many_kernel<128>, blocks, MANY_THREADS, Many<128>::SMEM, s, a, few, tk, tv);
-    } else {
-        cudaFuncSetAttribute(pattn_many_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<64>::SMEM);
-        launch(pattn_many_kernel<64>, blocks, MANY_THREADS, Many<64>::SMEM, s, a, few, tk, tv);
-    }
+    cudaFuncSetAttribute(pattn_many_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<HD>::SMEM);
+    launch(pattn_many_kernel<HD, WIDE>, blocks, MANY_THREADS, Many<HD>::SMEM, s, a, tk, tv);
     launch_pattn_merge(s, a, (int) blocks, MANY_COLS);
     count_launch(2);
+}
+
+void launch_pattn_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
+    const bool wide = a.p.page >= MANY_KEYS;
+    if (a.p.hd == 128) { if (wide) launch_many<128, true>(s, a, tk, tv); else launch_many<128, false>(s, a, tk, tv); }
+    else if (wide) launch_many<64, true>(s, a, tk, tv);
+    else launch_many<64, false>(s, a, tk, tv);
 }
 
 }   // namespace nsl
