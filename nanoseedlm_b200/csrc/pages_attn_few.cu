@@ -92,12 +92,6 @@ __device__ __forceinline__ uint32_t few_turn(uint32_t x) {      // an 8 x 8 tile
     return r;
 }
 __device__ __forceinline__ void few_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_WARPS) : "memory"); }      // the computing warps
-__device__ __forceinline__ bool few_sync_any(bool x) {      // the same; whether any thread's x is true
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"((uint32_t) x), "n"(32 * FEW_WARPS) : "memory");
-    return r != 0;
-}
 
 // Column c's weights of the warps' states: cw[w * CT + c] = 2^(mo_w - mo); and m, l, mo of all.
 template <int HD, int CT>
@@ -169,18 +163,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
     FewWalk walk = {plan[0], plan[1]};
     FewItem it;
     int stage = 0, round = 0;      // the ring's next stage, and how often it has been round
-    volatile int* const ab = &abort_flag;
-    auto fail = [&](int code) { abort_flag = 1; atomicCAS(&g_pattn_status, 0, code); };
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) { pa_bar_wait(bar, parity, &abort_flag, &g_pattn_status, code); };
     const int piece = min(a.p.page, FEW_KEYS), pieces = FEW_KEYS / piece;      // rows of a piece, pieces of a unit
 
     if (warp == FEW_WARPS) {      // ---- fetches ----
         asm volatile("fence.proxy.async;" ::: "memory");      // codes that the kernel before has stored
         const int batch = 32 / pieces;      // units a look ahead covers
         int x = x0;
-        bool ok = true;
-        while (ok && walk.next(a, group, x, xe, &it)) {
+        while (walk.next(a, group, x, xe, &it)) {
             const size_t head_at = (size_t) a.layer * a.p.n_pages * a.p.n_kv + it.kvh;
-            for (int b = it.x0; ok && b < it.x1; b += batch) {
+            for (int b = it.x0; b < it.x1; b += batch) {
                 // lane j: piece j from position p on
                 const int p = (it.tile0 + b - it.first) * FEW_KEYS + lane * piece;
                 int id = -1;
@@ -193,7 +185,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
                 }
                 const int row = id < 0 ? -1 : (int) ((head_at + (size_t) id * a.p.n_kv) * a.p.page + p % a.p.page);
                 for (int u = 0; u < batch && b + u < it.x1; ++u) {
-                    if (round > 0 && !pa_bar_wait(empty + 8 * stage, (round - 1) & 1, ab)) { fail(1); ok = false; break; }
+                    if (round > 0) wait(empty + 8 * stage, (round - 1) & 1, 1);
+                    if (*(volatile int*) &abort_flag) break;
                     const int from = u * pieces + (lane & (pieces - 1)), of_group = u * pieces + (lane & 3) * 16 / piece;
                     const int my_row = __shfl_sync(0xFFFFFFFFu, row, from), g_row = __shfl_sync(0xFFFFFFFFu, row, of_group);
                     const float g_ks = __shfl_sync(0xFFFFFFFFu, ks, of_group), g_lv = __shfl_sync(0xFFFFFFFFu, lv, of_group);
@@ -212,11 +205,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
             }
             x = it.x1;
         }
-        if (!ok) {      // what is in flight ends before the block does
-            for (int i = 0; i < F::STAGES; ++i) {
-                const int filled = i < stage ? round + 1 : round;      // fills of stage i
-                if (filled > 0) for (uint32_t t = 0; t < (1u << 20) && !pa_bar_try(full + 8 * i, (filled - 1) & 1); ++t) {}
-            }
+        for (int i = 0; i < F::STAGES; ++i) {      // what is in flight ends before the block does, whatever the others do
+            const int filled = round + (i < stage);      // fills of stage i
+            if (filled > 0) for (uint32_t k = 0; k < (1u << 20) && !pa_bar_try(full + 8 * i, (filled - 1) & 1); ++k) {}
         }
         return;
     }
@@ -276,9 +267,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) ot[nt][i][0] = ot[nt][i][1] = ot[nt][i][2] = ot[nt][i][3] = 0.0f;
         }
-        bool failed = false;
         for (x = it.x0; x < it.x1; ++x) {
-            if (!pa_bar_wait(full + 8 * stage, round & 1, ab)) { fail(2); failed = true; break; }
+            wait(full + 8 * stage, round & 1, 2);
             const float4 mt = meta[4 * stage + warp];
             const int key = (it.tile0 + x - it.first) * FEW_KEYS + 16 * warp;
             if (mt.z != 0.0f && key < it.k1 && key + 16 > it.k0) {
@@ -351,7 +341,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
             if (++stage == F::STAGES) { stage = 0; ++round; }
         }
         // the warps' states side by side, merged into the block's
-        if (few_sync_any(failed)) return;      // (the last item's states have been read)
+        few_sync();      // the last item's states have been read
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

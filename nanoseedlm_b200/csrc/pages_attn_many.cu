@@ -6,8 +6,8 @@
 //   S [128][64]  = Q [128][hd] . K^T      A = queries (f16; the first tile's in tensor memory, the second's in shared memory), B = keys [64][hd]
 //   O [128][hd] += W [128][64] . V        A = weights (f16, tensor memory), B = values as [hd][64]
 // Warps: 4 + 4 take the softmax of the two tiles (a thread a column: its row of S is in its tensor memory lane), 4 expand the
-// codes to f16 (exact) into the layout the products read, 1 fetches pages, 1 issues the products: the scores of a tile's next
-// unit as soon as the last ones are in registers, the values once the weights are there.  An item of up to 128 columns has both
+// codes to f16 (exact) into the layout the products read, 1 fetches pages, 1 issues the scores' products (a tile's next unit as
+// soon as the last scores are in registers), 1 the values' (once the weights are there).  An item of up to 128 columns has both
 // tiles work on the same queries, every other unit each, and their states joined at its end.
 // The two scales and the running maxima are as in pages_attn_few.cu; here the maxima that the exponents use follow the true ones
 // only when these have grown by 2^8 (weights up to 2^8 then), so O in tensor memory is hardly ever rescaled.
@@ -20,8 +20,8 @@
 
 namespace nsl {
 
-constexpr int MANY_KEYS = 64, MANY_TILE = 128, MANY_COLS = PATTN_MANY, MANY_THREADS = 448, MANY_RAW = 3, MANY_STAGES = 4, MANY_META = 16;
-constexpr int MANY_EXPAND = 8, MANY_FETCH = 12, MANY_MMA = 13;      // first warp of each part; the softmax has warps 0 .. 7
+constexpr int MANY_KEYS = 64, MANY_TILE = 128, MANY_COLS = PATTN_MANY, MANY_THREADS = 480, MANY_RAW = 3, MANY_STAGES = 4, MANY_META = 16;
+constexpr int MANY_EXPAND = 8, MANY_FETCH = 12, MANY_SCORES = 13, MANY_VALUES = 14;      // first warp of each part; the softmax has warps 0 .. 7
 constexpr int TM_S = 0, TM_Q = 128, TM_W = 192, TM_O = 256;         // tensor memory columns: S (64 a tile), the first tile's Q (64), W (32 a tile), O (128 a tile)
 constexpr float MANY_SLACK = 8.0f;                                   // how far (in powers of 2) a weight may exceed 1
 
@@ -150,11 +150,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ bool softmax_sync(bool x) {      // the softmax warps of both tiles; whether any thread's x is true
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((uint32_t) x) : "memory");
-    return r != 0;
-}
+__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }      // the softmax warps of both tiles
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void many_ldsm_trans(uint32_t* r, uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -185,7 +181,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
     const uint32_t base = pa_smem(smem), tiles = base + F::OFF_TILES, bars = base + F::OFF_BARS;
     // arrivals: raw_full the fetch (and bytes), raw_empty the 4 expanding warps, tile_full the same, tile_empty the products, meta the fetch;
     // per tile: s_full and o_done (a unit's scores are there, its values are in O) the products, s_free (the scores are in registers),
-    // w_full and q_full the tile's 4 warps; done the products
+    // w_full and q_full the tile's 4 warps; done the warps that issue products
     const uint32_t raw_full = bars, raw_empty = raw_full + 8 * MANY_RAW, tile_full = raw_empty + 8 * MANY_RAW, tile_empty = tile_full + 8 * MANY_STAGES, meta_full = tile_empty + 8 * MANY_STAGES,
                    s_full = meta_full + 8 * MANY_META, s_free = s_full + 16, w_full = s_free + 16, q_full = w_full + 16, o_done = q_full + 16, done = o_done + 16;
     const float4* const meta = (const float4*) (smem + F::OFF_META);
@@ -194,12 +190,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
         for (int i = 0; i < MANY_STAGES; ++i) { pa_bar_init(tile_full + 8 * i, 4); pa_bar_init(tile_empty + 8 * i, 1); }
         for (int i = 0; i < MANY_META; ++i) pa_bar_init(meta_full + 8 * i, 1);
         for (int t = 0; t < 2; ++t) { pa_bar_init(s_full + 8 * t, 1); pa_bar_init(s_free + 8 * t, 4); pa_bar_init(w_full + 8 * t, 4); pa_bar_init(q_full + 8 * t, 4); pa_bar_init(o_done + 8 * t, 1); }
-        pa_bar_init(done, 1);
+        pa_bar_init(done, 2);
         abort_flag = 0;
         plan[0] = plan[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == MANY_MMA) {
+    if (warp == MANY_SCORES) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pa_smem(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -246,9 +242,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
     __syncthreads();
     ManyWalk walk = {plan[0], plan[1]};
     ManyItem it;
-    volatile int* const ab = &abort_flag;
-    bool ok = tmem_slot == tmem;      // (it is: nothing else can have been allocated)
-    auto fail = [&](int code) { abort_flag = 1; atomicCAS(&g_pattn_many_status, 0, code); ok = false; };
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) { pa_bar_wait(bar, parity, &abort_flag, &g_pattn_many_status, code); };
     int g = 0;      // units this block has done: the rings' position
 
     if (warp < MANY_EXPAND) {      // ---- softmax: tile t, column c of it ----
@@ -306,11 +300,13 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
             float m = -INFINITY, mo = -INFINITY, l = 0.0f;
             for (int j = 0; j < n; ++j, ++steps) {
                 const int u = shared ? 2 * j + t : j, at = g + u;      // the unit; its place in the rings
-                if (!pa_bar_wait(s_full + 8 * t, steps & 1, ab) || !pa_bar_wait(meta_full + 8 * (at % MANY_META), at / MANY_META & 1, ab)) { fail(4); break; }
+                wait(s_full + 8 * t, steps & 1, 4);
+                wait(meta_full + 8 * (at % MANY_META), at / MANY_META & 1, 5);
                 tm_after();
-                if (!warp_valid) {
-                    __syncwarp();
-                    if (lane == 0) { pa_bar_arrive(s_free + 8 * t); pa_bar_arrive(w_full + 8 * t); }
+                if (!warp_valid) {      // (the last unit's arrivals are complete once its values are in O)
+                    if (lane == 0) pa_bar_arrive(s_free + 8 * t);
+                    if (j > 0) wait(o_done + 8 * t, (steps - 1) & 1, 6);
+                    if (lane == 0) pa_bar_arrive(w_full + 8 * t);
                     continue;
                 }
                 uint32_t su[64];
@@ -354,23 +350,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                 if (mn > m + MANY_SLACK || (m == -INFINITY && mn > m)) { l *= pa_ex2(m - mn); m = mn; }
                 const bool up = mon > mo + MANY_SLACK || (mo == -INFINITY && mon > mo);
                 const bool any_up = __any_sync(0xFFFFFFFFu, up);
-                // the tile's last values are in O, and its last weights have been read
-                if (j > 0 && !pa_bar_wait(o_done + 8 * t, (steps - 1) & 1, ab)) { fail(5); break; }
-                if (any_up) {
-                    const float cor = up ? pa_ex2(mo - mon) : 1.0f;
-                    if (up) mo = mon;
-                    if (j > 0) {
-                        tm_after();
-#pragma unroll 1
-                        for (int d = 0; d < HD; d += 16) {
-                            uint32_t v[16];
-                            tm_ld16(to + d, v);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * cor);
-                            tm_st16(to + d, v);
-                        }
-                    }
-                }
+                float cor = 1.0f;
+                if (up) { cor = pa_ex2(mo - mon); mo = mon; }
                 const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
                 // a weight is p cf, p = 2^(score - m), cf = 2^lc: one exponential of the sum, p's sum from the weights' sum, unless
                 // the two lie so far apart that a weight underflows where its p counts
@@ -378,10 +359,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                 bool near = true;
 #pragma unroll
                 for (int i = 0; i < NG; ++i) { lc[i] = lv[i] + (ms - mos); near = near && fabsf(lc[i]) <= 64.0f; }
+                uint32_t w[32];
                 if (__all_sync(0xFFFFFFFFu, near)) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        uint32_t w[16];
 #pragma unroll
                         for (int i = WIDE ? 0 : 2 * h; i < (WIDE ? 1 : 2 * h + 2); ++i) {
                             const u64 f2 = pack2(fg[i], fg[i]), b2 = pack2(lc[i] - ms, lc[i] - ms);
@@ -394,43 +375,54 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                                 unpack2(fma2(pack2(s[e0 + 2 * e], s[e0 + 2 * e + 1]), f2, b2), w0, w1);
                                 w0 = pa_ex2(w0); w1 = pa_ex2(w1);
                                 sum = add2(sum, pack2(w0, w1));
-                                w[e0 / 2 - 16 * h + e] = pa_f16x2(w0, w1);
+                                w[e0 / 2 + e] = pa_f16x2(w0, w1);
                             }
                             float l0, l1;
                             unpack2(sum, l0, l1);
                             l = fmaf(l0 + l1, pa_ex2(-lc[i]), l);
                         }
-                        tm_st16(tw + 16 * h, w);
                     }
                 } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int k = 32 * h + 2 * e, i = k / GK;
-                            const float cf = pa_ex2(fminf(lc[i], 120.0f));      // finite: a weight whose p is 0 is 0
-                            const float p0 = pa_ex2(fmaf(s[k], fg[i], -ms)), p1 = pa_ex2(fmaf(s[k + 1], fg[i], -ms));
-                            l += p0 + p1;
-                            w[e] = pa_f16x2(p0 * cf, p1 * cf);
-                        }
-                        tm_st16(tw + 16 * h, w);
+                    for (int e = 0; e < 32; ++e) {
+                        const int i = 2 * e / GK;
+                        const float cf = pa_ex2(fminf(lc[i], 120.0f));      // finite: a weight whose p is 0 is 0
+                        const float p0 = pa_ex2(fmaf(s[2 * e], fg[i], -ms)), p1 = pa_ex2(fmaf(s[2 * e + 1], fg[i], -ms));
+                        l += p0 + p1;
+                        w[e] = pa_f16x2(p0 * cf, p1 * cf);
                     }
                 }
+                // the tile's last values are in O, and its last weights have been read
+                if (j > 0) {
+                    wait(o_done + 8 * t, (steps - 1) & 1, 6);
+                    if (any_up) {
+                        tm_after();
+#pragma unroll 1
+                        for (int d = 0; d < HD; d += 16) {
+                            uint32_t v[16];
+                            tm_ld16(to + d, v);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * cor);
+                            tm_st16(to + d, v);
+                        }
+                    }
+                }
+                tm_st16(tw, w);
+                tm_st16(tw + 16, w + 16);
                 tm_wait_st();
                 tm_before();
                 __syncwarp();
                 if (lane == 0) pa_bar_arrive(w_full + 8 * t);
             }
-            if (ok && n > 0 && !pa_bar_wait(o_done + 8 * t, (steps - 1) & 1, ab)) fail(5);
+            if (n > 0) wait(o_done + 8 * t, (steps - 1) & 1, 6);
             // ---- results ----
             const int b0 = it.first / per, parts = (it.first + it.units - 1) / per - b0 + 1;
             float by = 1.0f, by1 = 0.0f;      // what this tile's and the second's O are multiplied with
             if (shared && t == 1) { other[0][c] = m; other[1][c] = l; other[2][c] = mo; }
-            tm_before();
-            if (softmax_sync(!ok)) { ok = false; break; }      // (all eight warps stay together, whatever fails)
-            tm_after();
             if (shared) {
+                tm_before();
+                softmax_sync();
+                tm_after();
                 if (t == 0) {
                     const float m1 = other[0][c], mo1 = other[2][c], mm = fmaxf(m, m1), mmo = fmaxf(mo, mo1);
                     const float ms = mm == -INFINITY ? 0.0f : mm, mos = mmo == -INFINITY ? 0.0f : mmo;
@@ -468,7 +460,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
             }
             if (shared) {      // the second tile's O has been read
                 tm_before();
-                softmax_sync(false);
+                softmax_sync();
                 tm_after();
             }
             if (tid == 0 && parts > 1 && (int) blockIdx.x == b0) a.rec[blockIdx.x] = make_int4(parts | it.kvh << 16, it.sp.row, it.col0, it.cols);
@@ -483,9 +475,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
         const uint32_t v_from = (uint32_t) F::RAW + (uint32_t) (16 * w + lrow) * HD, v_x = (uint32_t) (lane >> 4) ^ sw;
         const int odd = lane >> 4, half = lane >> 3 & 1;
         const uint32_t v_to = (uint32_t) F::TILE + (uint32_t) (8 * odd + (lane & 7)) * 128 + (((uint32_t) (2 * w + half) ^ (uint32_t) (lane & 7)) << 4);
-        for (int n = xe - x0; ok && g < n; ++g) {
+        for (int n = xe - x0; g < n; ++g) {
             const uint32_t rs = (uint32_t) (g % MANY_RAW), st = (uint32_t) (g % MANY_STAGES);
-            if (!pa_bar_wait(raw_full + 8 * rs, g / MANY_RAW & 1, ab) || (g >= MANY_STAGES && !pa_bar_wait(tile_empty + 8 * st, (g / MANY_STAGES - 1) & 1, ab))) { fail(6); break; }
+            wait(raw_full + 8 * rs, g / MANY_RAW & 1, 7);
+            if (g >= MANY_STAGES) wait(tile_empty + 8 * st, (g / MANY_STAGES - 1) & 1, 8);
             const uint32_t raw = base + rs * 2 * F::RAW, out = tiles + st * 2 * F::TILE;
             // keys: row and chunk of 16 codes a thread -> two 16-byte pieces of the row's f16 values
 #pragma unroll
@@ -523,9 +516,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
         asm volatile("fence.proxy.async;" ::: "memory");      // codes that the kernel before has stored
         const int piece = min(a.p.page, MANY_KEYS), pieces = MANY_KEYS / piece, batch = 32 / pieces;
         float4* const meta_to = (float4*) (smem + F::OFF_META);
-        for (int x = x0; ok && walk.next(a, group, x, xe, &it); x = it.x1) {
+        for (int x = x0; walk.next(a, group, x, xe, &it); x = it.x1) {
             const size_t head_at = (size_t) a.layer * a.p.n_pages * a.p.n_kv + it.kvh;
-            for (int b = it.x0; ok && b < it.x1; b += batch) {
+            for (int b = it.x0; b < it.x1; b += batch) {
                 const int p = (it.tile0 + b - it.first) * MANY_KEYS + lane * piece;      // lane j: piece j from here on
                 int id = -1;
                 float ks = 0.0f, lv = 0.0f;
@@ -538,7 +531,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                 const int row = id < 0 ? -1 : (int) ((head_at + (size_t) id * a.p.n_kv) * a.p.page + p % a.p.page);
                 for (int u = 0; u < batch && b + u < it.x1; ++u, ++g) {
                     const uint32_t rs = (uint32_t) (g % MANY_RAW);
-                    if (g >= MANY_RAW && !pa_bar_wait(raw_empty + 8 * rs, (g / MANY_RAW - 1) & 1, ab)) { fail(7); break; }
+                    if (g >= MANY_RAW) wait(raw_empty + 8 * rs, (g / MANY_RAW - 1) & 1, 9);
+                    if (*(volatile int*) &abort_flag) break;
                     const int from = u * pieces + (lane & (pieces - 1)), of_group = u * pieces + (lane & 3) * 16 / piece;
                     const int my_row = __shfl_sync(0xFFFFFFFFu, row, from), g_row = __shfl_sync(0xFFFFFFFFu, row, of_group);
                     const float g_ks = __shfl_sync(0xFFFFFFFFu, ks, of_group), g_lv = __shfl_sync(0xFFFFFFFFu, lv, of_group);
@@ -558,28 +552,31 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                 }
             }
         }
-        if (!ok)      // what is in flight ends before the block does
-            for (int i = 0; i < MANY_RAW; ++i) {
-                const int filled = g / MANY_RAW + (i < g % MANY_RAW);
-                if (filled > 0) for (uint32_t k = 0; k < (1u << 20) && !pa_bar_try(raw_full + 8 * i, (filled - 1) & 1); ++k) {}
-            }
-    } else {      // ---- issues the products ----
+        for (int i = 0; i < MANY_RAW; ++i) {      // what is in flight ends before the block does, whatever the others do
+            const int filled = g / MANY_RAW + (i < g % MANY_RAW);
+            if (filled > 0) for (uint32_t k = 0; k < (1u << 20) && !pa_bar_try(raw_full + 8 * i, (filled - 1) & 1); ++k) {}
+        }
+    } else {      // ---- issues the products: the scores', or the values' ----
         // everything that an operand is made of comes from constants, counters and values that the warp is known to share (same())
         constexpr uint32_t id_s = many_idesc(MANY_KEYS), id_o = many_idesc(HD);
+        const bool scores = warp == MANY_SCORES;
         const uint64_t qd = many_desc(base + F::OFF_Q), kd0 = many_desc(tiles), vd0 = many_desc(tiles + F::TILE);
-        uint32_t items = 0, units = 0, scored[2] = {0, 0}, summed[2] = {0, 0};      // of this block so far; of a tile: units scored, values added
-        for (int x = x0; ok && walk.next(a, group, x, xe, &it); x = it.x1, ++items) {
+        uint32_t items = 0, units = 0, issued[2] = {0, 0};      // of this block so far; of a tile: units
+        for (int x = x0; walk.next(a, group, x, xe, &it); x = it.x1, ++items) {
             const uint32_t run = same(it.x1 - it.x0), shared = same(it.cols <= MANY_TILE), n = shared ? run : 2 * run;
-            if (!pa_bar_wait(q_full, items & 1, ab) || !pa_bar_wait(q_full + 8, items & 1, ab)) { fail(8); break; }
-            tm_after();
-            // step i: the scores of tile i & 1, then the values of its step before
-            auto step = [&](auto tile, uint32_t i) {
+            if (scores) {
+                wait(q_full, items & 1, 10);
+                wait(q_full + 8, items & 1, 10);
+                tm_after();
+            }
+            auto step = [&](auto tile, uint32_t i) {      // of tile i & 1
                 constexpr int t = decltype(tile)::value;
-                if (i < n) {
-                    const uint32_t at = units + (shared ? i : i >> 1), stage = at % MANY_STAGES;
-                    if (!pa_bar_wait(tile_full + 8 * stage, at / MANY_STAGES & 1, ab) || (scored[t] > 0 && !pa_bar_wait(s_free + 8 * t, (scored[t] - 1) & 1, ab))) { fail(9); return; }
+                if (i >= n) return;
+                const uint32_t at = units + (shared ? i : i >> 1), stage = at % MANY_STAGES;
+                if (scores) {
+                    wait(tile_full + 8 * stage, at / MANY_STAGES & 1, 11);
+                    if (issued[t] > 0) wait(s_free + 8 * t, (issued[t] - 1) & 1, 12);
                     tm_after();
-                    ++scored[t];
                     const uint64_t kd = kd0 + (uint64_t) (stage * (2 * F::TILE >> 4));
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
@@ -588,22 +585,20 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                         else many_mma_smem(TM_S + 64, qd + (uint64_t) (((k >> 2) * (MANY_TILE * 128) + (k & 3) * 32) >> 4), kk, id_s, k > 0);
                     }
                     many_commit(s_full + 8 * t);
-                }
-                if (i >= 2 && i < n + 2) {
-                    const uint32_t at = units + (shared ? i - 2 : (i - 2) >> 1), stage = at % MANY_STAGES;
-                    if (!pa_bar_wait(w_full + 8 * t, summed[t] & 1, ab)) { fail(10); return; }
+                } else {
+                    wait(w_full + 8 * t, issued[t] & 1, 13);
                     tm_after();
-                    ++summed[t];
                     const uint64_t vd = vd0 + (uint64_t) (stage * (2 * F::TILE >> 4));
 #pragma unroll
-                    for (int k = 0; k < MANY_KEYS / 16; ++k) many_mma(TM_O + 128 * t, TM_W + 32 * t + 8 * k, vd + (uint64_t) (2 * k), id_o, i >= 4 || k > 0);
+                    for (int k = 0; k < MANY_KEYS / 16; ++k) many_mma(TM_O + 128 * t, TM_W + 32 * t + 8 * k, vd + (uint64_t) (2 * k), id_o, i >= 2 || k > 0);
                     many_commit(o_done + 8 * t);
-                    if (shared || t == 1) many_commit(tile_empty + 8 * stage);
+                    if (shared || t == 1) many_commit(tile_empty + 8 * stage);      // (its keys were read before the weights could be made)
                 }
+                ++issued[t];
             };
-            for (uint32_t i = 0; ok && i < n + 2; i += 2) {
+            for (uint32_t i = 0; i < n; i += 2) {
                 step(std::integral_constant<int, 0>(), i);
-                if (ok) step(std::integral_constant<int, 1>(), i + 1);
+                step(std::integral_constant<int, 1>(), i + 1);
             }
             units += run;
         }
@@ -614,7 +609,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
     tm_before();
     __syncthreads();
     tm_after();
-    if (warp == MANY_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_slot) : "memory");
+    if (warp == MANY_SCORES) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_slot) : "memory");
 }
 
 int pattn_many_status() {
