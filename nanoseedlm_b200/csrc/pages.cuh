@@ -16,13 +16,15 @@ bool pages_ok(const NslPages* p, const char* who);      // pages.cu
 inline bool layer_ok(const NslPages* p, int layer) { return layer >= 0 && layer < p->n_layer; }
 
 #ifdef __CUDACC__
+__device__ __forceinline__ void eight_of(const uint4& u, float* x) {      // packed bf16
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+}
 template <int TYPE>
 __device__ __forceinline__ void load8(const void* base, size_t at, float* x) {
     if (TYPE == NSL_BF16) {
-        const uint4 u = *(const uint4*) ((const uint16_t*) base + at);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+        eight_of(*(const uint4*) ((const uint16_t*) base + at), x);
     } else {
         const float4 a = *(const float4*) ((const float*) base + at), b = *(const float4*) ((const float*) base + at + 4);
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;

@@ -3,40 +3,76 @@
 
 namespace nsl {
 
-// An item's states joined.  Block (b, y): the item that block b of the first pass leaves unfinished, every gridDim.y-th pair of its
-// columns; a warp takes every fourth state of a column, four dims a lane (HD = 64: half the lanes).
-constexpr int MERGE_THREADS = 256, MERGE_EACH = MERGE_THREADS / 32 / 2;
+// An item's states joined.  Block (b, y): the item that block b of the first pass leaves unfinished, some of its columns.  Up to
+// MERGE_FEW states: a warp a column, everything requested before anything is used; more: four warps a column, every fourth state
+// each.  Bound: latency (a prompt's call of 148 unfinished items of 256 columns moves 80 MB through L2).
+constexpr int MERGE_THREADS = 256, MERGE_WARPS = MERGE_THREADS / 32, MERGE_EACH = 4, MERGE_FEW = 4;
+
+template <int HD>
+__device__ __forceinline__ void merge_store(const PagesAttn& a, const int4& rec, int col, int lane, float4 o, float f) {
+    const int group = a.n_head / a.p.n_kv, c = rec.z + col, kvh = rec.x >> 16;
+    const size_t at = (size_t) (rec.y + c / group) * a.o_stride + (size_t) (kvh * group + c % group) * HD + 4 * lane;
+    const uint32_t lo = bf16_pair(o.x * f, o.y * f), hi = bf16_pair(o.z * f, o.w * f);
+    if (a.o_type == NSL_BF16) *(uint2*) ((uint16_t*) a.o + at) = make_uint2(lo, hi);
+    else *(float4*) ((float*) a.o + at) = make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xFFFF0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xFFFF0000u));
+}
+__device__ __forceinline__ void merge_add(float4& o, const float4& v, float w) {
+    o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
+}
+__device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.0f : m; }
+
 template <int HD>
 __global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a, int most_cols) {
     constexpr int STATE = PATTN_STATE<HD>;
-    __shared__ float4 sum[MERGE_THREADS / 32][32];
-    __shared__ float stat[MERGE_THREADS / 32][3];
+    __shared__ float4 sum[MERGE_WARPS][32];
+    __shared__ float stat[MERGE_WARPS][3];
     grid_dependents_go();
     grid_dependency_wait();
     const int4 rec = a.rec[blockIdx.x];
-    const int parts = rec.x & 0xFFFF, kvh = rec.x >> 16, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, turn = warp % MERGE_EACH;
+    const int parts = rec.x & 0xFFFF, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (parts == 0) return;
-    for (int pair = blockIdx.y; 2 * pair < rec.w; pair += gridDim.y) {
-        const int col = 2 * pair + warp / MERGE_EACH;
-        __syncthreads();      // the last pair's sums have been read
+    auto state = [&](int i, int col) { return a.part + ((size_t) (2 * ((int) blockIdx.x + i) + (i == 0)) * most_cols + col) * STATE; };
+    if (parts <= MERGE_FEW) {
+        for (int col = (int) blockIdx.y * MERGE_WARPS + warp; col < rec.w; col += (int) gridDim.y * MERGE_WARPS) {
+            float4 v[MERGE_FEW], st[MERGE_FEW];
+#pragma unroll
+            for (int i = 0; i < MERGE_FEW; ++i) {
+                const float* p = state(min(i, parts - 1), col);
+                st[i] = *(const float4*) (p + HD);
+                v[i] = *(const float4*) (p + 4 * (4 * lane < HD ? lane : 0));
+                if (i >= parts) st[i] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+            }
+            float m = -INFINITY, mo = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < MERGE_FEW; ++i) { m = fmaxf(m, st[i].x); mo = fmaxf(mo, st[i].z); }
+            const float ms = finite_or_0(m), mos = finite_or_0(mo);
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < MERGE_FEW; ++i)
+                if (i < parts) { l = fmaf(st[i].y, pa_ex2(st[i].x - ms), l); merge_add(o, v[i], pa_ex2(st[i].z - mos)); }
+            if (4 * lane < HD) merge_store<HD>(a, rec, col, lane, o, pattn_factor(m, l, mo));
+        }
+        return;
+    }
+    const int turn = warp % MERGE_EACH;
+    constexpr int COLS = MERGE_WARPS / MERGE_EACH;
+    for (int c0 = (int) blockIdx.y * COLS; c0 < rec.w; c0 += (int) gridDim.y * COLS) {
+        const int col = c0 + warp / MERGE_EACH;
+        __syncthreads();      // the last columns' sums have been read
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float m = -INFINITY, mo = -INFINITY, l = 0.0f;
-        auto state = [&](int i) { return a.part + ((size_t) (2 * ((int) blockIdx.x + i) + (i == 0)) * most_cols + col) * STATE; };
         if (col < rec.w) {
             // the maxima over this warp's states, a state a lane; then the sums
-            for (int i = turn + MERGE_EACH * lane; i < parts; i += MERGE_EACH * 32) { m = fmaxf(m, state(i)[HD]); mo = fmaxf(mo, state(i)[HD + 2]); }
+            for (int i = turn + MERGE_EACH * lane; i < parts; i += MERGE_EACH * 32) { const float* st = state(i, col) + HD; m = fmaxf(m, st[0]); mo = fmaxf(mo, st[2]); }
 #pragma unroll
             for (int x = 16; x > 0; x >>= 1) { m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x)); mo = fmaxf(mo, __shfl_xor_sync(0xFFFFFFFFu, mo, x)); }
-            const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
+            const float ms = finite_or_0(m), mos = finite_or_0(mo);
 #pragma unroll 8
             for (int i = turn; i < parts; i += MERGE_EACH) {
-                const float* st = state(i);
-                const float w = pa_ex2(st[HD + 2] - mos);
-                l = fmaf(st[HD + 1], pa_ex2(st[HD] - ms), l);
-                if (4 * lane < HD) {
-                    const float4 v = *(const float4*) (st + 4 * lane);
-                    o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
-                }
+                const float* p = state(i, col);
+                const float4 st = *(const float4*) (p + HD);
+                l = fmaf(st.y, pa_ex2(st.x - ms), l);
+                if (4 * lane < HD) merge_add(o, *(const float4*) (p + 4 * lane), pa_ex2(st.z - mos));
             }
         }
         sum[warp][lane] = o;
@@ -44,27 +80,22 @@ __global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a,
         __syncthreads();
         if (turn || col >= rec.w || 4 * lane >= HD) continue;
         for (int w = 1; w < MERGE_EACH; ++w) { m = fmaxf(m, stat[warp + w][0]); mo = fmaxf(mo, stat[warp + w][2]); }
-        const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo;
+        const float ms = finite_or_0(m), mos = finite_or_0(mo);
         o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         l = 0.0f;
 #pragma unroll
         for (int w = 0; w < MERGE_EACH; ++w) {
-            const float4 v = sum[warp + w][lane];
-            const float by = pa_ex2(stat[warp + w][2] - mos);
             l = fmaf(stat[warp + w][1], pa_ex2(stat[warp + w][0] - ms), l);
-            o.x = fmaf(v.x, by, o.x); o.y = fmaf(v.y, by, o.y); o.z = fmaf(v.z, by, o.z); o.w = fmaf(v.w, by, o.w);
+            merge_add(o, sum[warp + w][lane], pa_ex2(stat[warp + w][2] - mos));
         }
-        const int group = a.n_head / a.p.n_kv, c = rec.z + col;
-        const float f = pattn_factor(m, l, mo);
-        const size_t at = (size_t) (rec.y + c / group) * a.o_stride + (size_t) (kvh * group + c % group) * HD + 4 * lane;
-        const uint32_t lo = bf16_pair(o.x * f, o.y * f), hi = bf16_pair(o.z * f, o.w * f);
-        if (a.o_type == NSL_BF16) *(uint2*) ((uint16_t*) a.o + at) = make_uint2(lo, hi);
-        else *(float4*) ((float*) a.o + at) = make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xFFFF0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xFFFF0000u));
+        merge_store<HD>(a, rec, col, lane, o, pattn_factor(m, l, mo));
     }
 }
 
 void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks, int most_cols) {
-    const dim3 grid((unsigned) blocks, (unsigned) (most_cols / 2 < 16 ? most_cols / 2 : 16));
+    const int cols = (a.n_head / a.p.n_kv) * (a.max_rows < a.T ? a.max_rows : a.T);      // (checked to fit before the first pass)
+    const int some = cols < most_cols ? cols : most_cols;
+    const dim3 grid((unsigned) blocks, (unsigned) (some <= PATTN_FEW ? (some + 1) / 2 : 32));
     if (a.p.hd == 128) launch(pattn_merge_kernel<128>, grid, MERGE_THREADS, 0, s, a, most_cols);
     else launch(pattn_merge_kernel<64>, grid, MERGE_THREADS, 0, s, a, most_cols);
 }
@@ -104,7 +135,7 @@ void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, co
                     const NslSeqRows* seqs, int n_seqs, int max_rows, int T, int o_type, void* o, int o_stride, void* work) {
     if (T <= 0 || n_seqs <= 0 || max_rows <= 0) return;
     if (!pages_ok(p, "nsl_pages_attn")) return;
-    if (!layer_ok(p, layer) || !known_type(q_type) || (o_type != NSL_BF16 && o_type != NSL_F32_BF16) || n_head < 1 || n_head % p->n_kv || n_head > 65535 || !seqs || n_seqs > 4096 ||
+    if (!layer_ok(p, layer) || !known_type(q_type) || (o_type != NSL_BF16 && o_type != NSL_F32_BF16) || n_head < 1 || n_head % p->n_kv || n_head > 65535 || (long long) n_head * T > 0x7FFFFFFF || !seqs || n_seqs > 4096 ||
         !work || !aligned16(work) || !rows_ok(q, q_stride, n_head * p->hd, q_type) || !rows_ok(o, o_stride, n_head * p->hd, o_type)) {
         set_error("nsl_pages_attn: layer %d of %d, types %d and %d, %d query heads over %d, %d sequences (at most 4096), or rows or work memory that are not 16-byte aligned", layer, p->n_layer,
                   q_type, o_type, n_head, p->n_kv, n_seqs);

@@ -369,8 +369,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
             } else mine[(size_t) c * STATE + d] = o;
         }
         if (parts > 1 && tid < cols) {
-            float* st = mine + (size_t) tid * STATE + HD;
-            st[0] = state_s[3 * tid]; st[1] = state_s[3 * tid + 1]; st[2] = state_s[3 * tid + 2];
+            *(float4*) (mine + (size_t) tid * STATE + HD) = make_float4(state_s[3 * tid], state_s[3 * tid + 1], state_s[3 * tid + 2], 0.0f);
         }
         if (tid == 0 && parts > 1 && (int) blockIdx.x == b0) a.rec[blockIdx.x] = make_int4(parts | it.kvh << 16, it.sp.row, 0, cols);
     }

@@ -65,7 +65,7 @@ __device__ __forceinline__ int warp_sum(int v) {
 // The walk over a block's units, by whole warps.
 struct ManyWalk {
     int i, before;
-    __device__ bool next(const PagesAttn& a, int group, int x, int xe, ManyItem* it) {
+    __device__ __noinline__ bool next(const PagesAttn& a, int group, int x, int xe, ManyItem* it) {
         const int lane = threadIdx.x & 31;
         if (x >= xe) return false;
         for (; i < a.n_seqs; ++i) {
@@ -167,9 +167,81 @@ __device__ __forceinline__ void many_sts(uint32_t at, uint32_t a, uint32_t b, ui
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// A column's query divided by its power of two, as f16 to tensor memory (tq) or, tq = 0, to its row of the shared panels of 64 dims
+// (at sq; sx: the row's swizzle).  -> |scale| log2 e times that power.  Requested whole where it fits the registers (bf16), for its
+// maximum first and then again otherwise.  Out of line, as its registers would be taken from the softmax.
+template <int HD>
+static __device__ __noinline__ float many_query(const PagesAttn& a, size_t at, bool valid, uint32_t tq, uint32_t sq, uint32_t sx) {
+    uint4 raw[HD / 8];
+    float top = 0.0f;
+    if (a.q_type == NSL_BF16) {
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) raw[j] = valid ? *(const uint4*) ((const uint16_t*) a.q + at + 8 * j) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) {
+            float v[8];
+            eight_of(raw[j], v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+        }
+    } else if (valid) {
+#pragma unroll 16
+        for (int d = 0; d < HD; d += 4) {
+            const float4 v = *(const float4*) ((const float*) a.q + at + d);
+            top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+        }
+    }
+    const float by = pa_pow2_of(top), inv = copysignf(1.0f / by, a.scale);      // the scale's sign goes with the query: maxima are then of scores
+#pragma unroll
+    for (int d = 0; d < HD; d += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float v[8];
+            if (a.q_type == NSL_BF16) eight_of(raw[d / 8 + j], v);
+            else if (valid) load8<NSL_F32>(a.q, at + d + 8 * j, v);
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[4 * j + e] = pa_f16x2(v[2 * e] * inv, v[2 * e + 1] * inv);
+            if (!tq) many_sts(sq + (d >> 6) * (MANY_TILE * 128) + (((uint32_t) ((d & 63) / 8 + j) ^ sx) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        }
+        if (tq) tm_st16(tq + d / 2, w);
+    }
+    if (tq) tm_wait_st();
+    else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    return fabsf(a.scale) * 1.4426950408889634f * by;
+}
+
+// A column's O (and, second: the other tile's, 128 columns on) out of tensor memory, times by and by1: to a state (part), or to the
+// results.  By whole warps.
+template <int HD>
+static __device__ __noinline__ void many_results(const PagesAttn& a, uint32_t to, bool second, float by, float by1, bool valid, float* part, size_t at) {
+#pragma unroll 1
+    for (int d = 0; d < HD; d += 16) {
+        uint32_t v[16], v1[16];
+        tm_ld16(to + d, v);
+        if (second) tm_ld16(to + 128 + d, v1);
+        if (!valid) continue;
+        // product row n = 16 j + r: dim 16 j + 2 r, n = 16 j + 8 + r: the next
+        float o[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float z = __uint_as_float(v[r]) * by;
+            if (second) z = fmaf(__uint_as_float(v1[r]), by1, z);
+            o[r < 8 ? 2 * r : 2 * (r - 8) + 1] = z;
+        }
+        if (part) { store8<NSL_F32>(part, d, o); store8<NSL_F32>(part, d + 8, o + 8); }
+        else if (a.o_type == NSL_BF16) { store8<NSL_BF16>(a.o, at + d, o); store8<NSL_BF16>(a.o, at + d + 8, o + 8); }
+        else { store8<NSL_F32_BF16>(a.o, at + d, o); store8<NSL_F32_BF16>(a.o, at + d + 8, o + 8); }
+    }
+}
+
 // WIDE: pages of 64 and more positions, a unit's keys have one pair of scales.
 template <int HD, bool WIDE>
-__global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
+__global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __grid_constant__ PagesAttn a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
     using F = Many<HD>;
     constexpr int STATE = PATTN_STATE<HD>, WARPS = MANY_THREADS / 32, NG = WIDE ? 1 : 4, GK = MANY_KEYS / NG;      // groups of GK keys with one pair of scales
     extern __shared__ uint8_t many_raw[];
@@ -257,39 +329,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
             const int hi = valid ? pos : -1, lo = valid && a.window > 0 ? pos - a.window + 1 : 0;
             float f = 0.0f;      // scale, log2 e and the power of two that the query is divided by
             if (warp_valid) {
-                float top = 0.0f;
-                const size_t at = (size_t) row * a.q_stride + (size_t) head * HD;
-                if (valid)
-#pragma unroll 4
-                    for (int d = 0; d < HD; d += 8) {
-                        float v[8];
-                        if (a.q_type == NSL_BF16) load8<NSL_BF16>(a.q, at + d, v); else load8<NSL_F32>(a.q, at + d, v);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
-                    }
-                const float by = pa_pow2_of(top), inv = copysignf(1.0f / by, a.scale);      // the scale's sign goes with the query: maxima are then of scores
-                f = fabsf(a.scale) * 1.4426950408889634f * by;
-#pragma unroll
-                for (int d = 0; d < HD; d += 32) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float v[8];
-                        if (!valid) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-                        } else if (a.q_type == NSL_BF16) load8<NSL_BF16>(a.q, at + d + 8 * j, v);
-                        else load8<NSL_F32>(a.q, at + d + 8 * j, v);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[4 * j + e] = pa_f16x2(v[2 * e] * inv, v[2 * e + 1] * inv);
-                        if (t == 1)      // panels of 64 dims, rows of 128 bytes
-                            many_sts(base + F::OFF_Q + (d >> 6) * (MANY_TILE * 128) + c * 128 + (((uint32_t) ((d & 63) / 8 + j) ^ (uint32_t) (c & 7)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2],
-                                     w[4 * j + 3]);
-                    }
-                    if (t == 0) tm_st16(lanes + TM_Q + d / 2, w);
-                }
-                if (t == 0) tm_wait_st();
-                else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                f = many_query<HD>(a, (size_t) row * a.q_stride + (size_t) head * HD, valid, t == 0 ? lanes + TM_Q : 0u, base + F::OFF_Q + c * 128, c & 7);
             }
             tm_before();
             __syncwarp();
@@ -434,28 +474,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(PagesAttn a
                 }
             }
             if (warp_valid && !(shared && t)) {
-                const float fac = parts == 1 ? pattn_factor(m, l, mo) : 1.0f;
-                const bool first = it.x1 - it.x0 > 0, second = shared && it.x1 - it.x0 > 1;      // (an O that nothing was added to holds anything)
+                const bool second = shared && it.x1 - it.x0 > 1;      // (an O that nothing was added to holds anything)
+                if (parts == 1) { const float fac = pattn_factor(m, l, mo); by *= fac; by1 *= fac; }
                 float* const part = a.part + ((size_t) (2 * blockIdx.x + ((int) blockIdx.x == b0)) * MANY_COLS + c0 + c) * STATE;
-                const size_t at = (size_t) row * a.o_stride + (size_t) head * HD;
-#pragma unroll 1
-                for (int d = 0; d < HD; d += 16) {
-                    uint32_t v[16], v1[16];
-                    tm_ld16(to + d, v);
-                    if (second) tm_ld16(to + 128 + d, v1);
-                    if (!valid) continue;
-                    // product row n = 16 j + r: dim 16 j + 2 r, n = 16 j + 8 + r: the next
-                    float o[16];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float z = first ? __uint_as_float(v[r]) * by : 0.0f;
-                        if (second) z = fmaf(__uint_as_float(v1[r]), by1, z);
-                        o[r < 8 ? 2 * r : 2 * (r - 8) + 1] = z * fac;
-                    }
-                    if (parts > 1) { store8<NSL_F32>(part, d, o); store8<NSL_F32>(part, d + 8, o + 8); }
-                    else if (a.o_type == NSL_BF16) { store8<NSL_BF16>(a.o, at + d, o); store8<NSL_BF16>(a.o, at + d + 8, o + 8); }
-                    else { store8<NSL_F32_BF16>(a.o, at + d, o); store8<NSL_F32_BF16>(a.o, at + d + 8, o + 8); }
-                }
+                many_results<HD>(a, to, second, by, by1, valid, parts > 1 ? part : NULL, (size_t) row * a.o_stride + (size_t) head * HD);
                 if (parts > 1 && valid) *(float4*) (part + HD) = make_float4(m, l, mo, 0.0f);
             }
             if (shared) {      // the second tile's O has been read
