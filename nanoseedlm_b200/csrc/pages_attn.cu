@@ -6,7 +6,7 @@ namespace nsl {
 // An item's states joined.  Block (b, y): the item that block b of the first pass leaves unfinished, some of its columns.  Up to
 // MERGE_FEW states: a warp a column, everything requested before anything is used; more: four warps a column, every fourth state
 // each.  Bound: latency (a prompt's call of 148 unfinished items of 256 columns moves 80 MB through L2).
-constexpr int MERGE_THREADS = 256, MERGE_WARPS = MERGE_THREADS / 32, MERGE_EACH = 4, MERGE_FEW = 4;
+constexpr int MERGE_THREADS = 256, MERGE_WARPS = MERGE_THREADS / 32, MERGE_EACH = 4, MERGE_FEW = 8;
 
 template <int HD>
 __device__ __forceinline__ void merge_store(const PagesAttn& a, const int4& rec, int col, int lane, float4 o, float f) {
@@ -37,10 +37,11 @@ __global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a,
             float4 v[MERGE_FEW], st[MERGE_FEW];
 #pragma unroll
             for (int i = 0; i < MERGE_FEW; ++i) {
-                const float* p = state(min(i, parts - 1), col);
+                st[i] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+                if (i >= parts) continue;
+                const float* p = state(i, col);
                 st[i] = *(const float4*) (p + HD);
                 v[i] = *(const float4*) (p + 4 * (4 * lane < HD ? lane : 0));
-                if (i >= parts) st[i] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
             }
             float m = -INFINITY, mo = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a,
 void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks, int most_cols) {
     const int cols = (a.n_head / a.p.n_kv) * (a.max_rows < a.T ? a.max_rows : a.T);      // (checked to fit before the first pass)
     const int some = cols < most_cols ? cols : most_cols;
-    const dim3 grid((unsigned) blocks, (unsigned) (some <= PATTN_FEW ? (some + 1) / 2 : 32));
+    const dim3 grid((unsigned) blocks, (unsigned) (some <= 64 ? (some + 1) / 2 : 32));
     if (a.p.hd == 128) launch(pattn_merge_kernel<128>, grid, MERGE_THREADS, 0, s, a, most_cols);
     else launch(pattn_merge_kernel<64>, grid, MERGE_THREADS, 0, s, a, most_cols);
 }

@@ -19,7 +19,7 @@ struct PagesAttn {
     int q_type, q_stride, o_type, o_stride, n_head, layer, window, n_seqs, max_rows, T;
 };
 
-// Blocks of a launch: two an SM (their number fits a record's 16 bits).
+// Blocks of a launch at most: two an SM (their number fits a record's 16 bits).
 inline int pattn_blocks() { return 2 * sm_count(); }
 constexpr int PATTN_FEW = 16, PATTN_MANY = 256;      // columns of an item
 template <int HD>
@@ -103,6 +103,19 @@ __device__ __forceinline__ float pa_query(const void* q, int type, size_t at) {
 __device__ __forceinline__ float pa_pow2_of(float x) {
     const int e = (int) (__float_as_uint(x) >> 23 & 0xFFu) - 127;
     return x == 0.0f ? 1.0f : __uint_as_float((uint32_t) (min(max(e, -126), 126) + 127) << 23);
+}
+
+// What the blocks' chains of dependent loads will come to (descriptors, page table, the layer's scales, queries), requested into L2 by all blocks
+// together before the wait for the kernel before: nothing is read, so what that still writes is not
+// missed.  A cold load costs 1 to 2 us here, and a block's first codes lie behind three of them.
+__device__ __forceinline__ void pattn_warm(const PagesAttn& a) {
+    const size_t scales = (size_t) a.layer * a.p.n_pages * a.p.n_kv, scale_lines = ((size_t) a.p.n_pages * a.p.n_kv * 4 + 127) / 128;
+    const char* const from[5] = {(const char*) a.seqs, (const char*) a.p.table, (const char*) (a.p.ks + scales), (const char*) (a.p.vs + scales), (const char*) a.q};
+    const size_t lines[5] = {((size_t) a.n_seqs * sizeof(NslSeqRows) + 127) / 128, ((size_t) a.p.n_seq * a.p.max_pages * 4 + 127) / 128, scale_lines, scale_lines, ((size_t) a.T * a.q_stride * (a.q_type == NSL_BF16 ? 2 : 4) + 127) / 128};
+    const size_t at = (size_t) blockIdx.x * blockDim.x + threadIdx.x;      // one line of each array a thread: 9 MB a launch
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+        if (at < lines[i]) asm volatile("prefetch.global.L2 [%0];" ::"l"(from[i] + 128 * at));
 }
 
 // A descriptor's rows that exist: [row, row + rows) of the call's rows, the first at position pos.

@@ -128,22 +128,22 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     grid_dependents_go();
+    pattn_warm(a);
     grid_dependency_wait();
-    // the step's units, and the descriptor that this block's first lies in
-    int total = 0, k0, k1;
-    for (int i = tid; i < a.n_seqs; i += FEW_THREADS) total += few_units(a, row_span(a, i), group, &k0, &k1) * a.p.n_kv;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-    if (lane == 0) wsum[warp] = total;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < FEW_THREADS / 32; ++w) total += wsum[w];
-    const int per = max((total + (int) gridDim.x - 1) / (int) gridDim.x, 1);
-    const int x0 = (int) blockIdx.x * per, xe = min(total, x0 + per);
-    if (tid == 0) a.rec[blockIdx.x] = make_int4(0, 0, 0, 0);      // (thread 0 writes it again below)
-    if (x0 >= xe) return;
+    // the step's units, and the descriptor that this block's first lies in: from one load of the descriptors where there is a thread for each
     if (tid == 0) { plan[0] = 0; plan[1] = 0; }
+    int total = 0, per = 0, x0 = 0, xe = 0, k0, k1;
+    const bool once = a.n_seqs <= FEW_THREADS;
+    if (!once) {
+        for (int i = tid; i < a.n_seqs; i += FEW_THREADS) total += few_units(a, row_span(a, i), group, &k0, &k1) * a.p.n_kv;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+        if (lane == 0) wsum[warp] = total;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < FEW_THREADS / 32; ++w) total += wsum[w];
+    }
     for (int base = 0, before = 0; base < a.n_seqs; base += FEW_THREADS) {
         const int i = base + tid, mine = i < a.n_seqs ? few_units(a, row_span(a, i), group, &k0, &k1) * a.p.n_kv : 0;
         int incl = mine;
@@ -155,11 +155,17 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
         int start = before + incl - mine, sum = 0;
 #pragma unroll
         for (int w = 0; w < FEW_THREADS / 32; ++w) { if (w < warp) start += wsum[w]; sum += wsum[w]; }
+        if (once) total = sum;
+        per = max((total + (int) gridDim.x - 1) / (int) gridDim.x, 1);
+        x0 = (int) blockIdx.x * per;
+        xe = min(total, x0 + per);
         if (mine && start <= x0 && x0 < start + mine) { plan[0] = i; plan[1] = start; }
         before += sum;
         if (before > x0) break;
     }
+    if (tid == 0) a.rec[blockIdx.x] = make_int4(0, 0, 0, 0);      // (thread 0 writes it again below)
     __syncthreads();
+    if (x0 >= xe) return;
     FewWalk walk = {plan[0], plan[1]};
     FewItem it;
     int stage = 0, round = 0;      // the ring's next stage, and how often it has been round
