@@ -11,7 +11,7 @@
 
 namespace nsl {
 
-constexpr int APPEND_THREADS = 256, APPEND_Q_ROWS = 4;
+constexpr int APPEND_THREADS = 256, APPEND_Q_ROWS = 8;      // APPEND_Q_ROWS: of a block at most
 
 // Pages that a descriptor's rows touch; rows outside [0, T) do not count.
 struct SeqSpan { int row, rows, pos; };
@@ -90,7 +90,7 @@ struct AppendArgs {
     void* qo;
     const NslSeqRows* seqs;
     int q_stride, qo_stride, k_stride, v_stride, n_head, layer, n_seqs, T;
-    int units, head_split, heads_each, kv_blocks;      // blocks: [units][2 tensors][head_split], then the query blocks
+    int units, head_split, heads_each, kv_blocks, q_rows;      // blocks: [units][2 tensors][head_split], then the query blocks of q_rows rows
 };
 
 // One (unit, tensor, heads) item.  GROUPS: groups of 16 values a thread holds (page * hd / 16 / threads at most).
@@ -167,20 +167,22 @@ __device__ void append_unit(const AppendArgs& a, int b, float2* cs) {
     }
 }
 
-// The queries of APPEND_Q_ROWS rows.
+// The queries of q_rows rows.
 template <int TYPE>
 __device__ void append_queries(const AppendArgs& a, int b, float2* cs) {
     __shared__ int found[APPEND_Q_ROWS], at[APPEND_Q_ROWS];
-    const int t0 = b * APPEND_Q_ROWS, pairs = a.r.rot / 2, hd = a.p.hd, groups = hd / 16;
-    for (int i = 0; i < APPEND_Q_ROWS; ++i) {
-        const int t = t0 + i, di = t < a.T ? row_descriptor(a.seqs, a.n_seqs, t, &found[i]) : -1;
-        if (threadIdx.x == 0) at[i] = di < 0 ? -1 : a.seqs[di].pos + (t - a.seqs[di].row);
+    const int t0 = b * a.q_rows, n = min(a.q_rows, a.T - t0), pairs = a.r.rot / 2, hd = a.p.hd, groups = hd / 16;
+    row_descriptors(a.seqs, a.n_seqs, t0, n, found);
+    if ((int) threadIdx.x < n) {
+        const int di = found[threadIdx.x];
+        at[threadIdx.x] = di < 0 ? -1 : a.seqs[di].pos + (t0 + (int) threadIdx.x - a.seqs[di].row);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < APPEND_Q_ROWS * pairs; i += APPEND_THREADS) cs[i] = rope_angle(max(at[i / pairs], 0), a.r.inv[i % pairs], a.r.factor);
+    for (int i = threadIdx.x; i < n * pairs; i += APPEND_THREADS) cs[i] = rope_angle(max(at[i / pairs], 0), a.r.inv[i % pairs], a.r.factor);
     __syncthreads();
     const int per_row = a.n_head * groups;
-    for (int i = threadIdx.x; i < APPEND_Q_ROWS * per_row; i += APPEND_THREADS) {
+#pragma unroll 2
+    for (int i = threadIdx.x; i < n * per_row; i += APPEND_THREADS) {
         const int row = i / per_row, g = i % groups, h = i % per_row / groups;
         if (at[row] < 0) continue;
         int ra, rb;
@@ -206,29 +208,29 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendArgs a) {
 }
 
 // Rows back: a thread takes 16 codes of a head.
-constexpr int READ_THREADS = 256, READ_ROWS = 4;
+constexpr int READ_THREADS = 256, READ_ROWS = 16;      // READ_ROWS: of a block at most
 template <int TYPE>
-__global__ void __launch_bounds__(READ_THREADS) read_kernel(NslPages p, int layer, void* ko, int ko_stride, void* vo, int vo_stride, const NslSeqRows* seqs, int n_seqs, int T) {
+__global__ void __launch_bounds__(READ_THREADS) read_kernel(NslPages p, int layer, void* ko, int ko_stride, void* vo, int vo_stride, const NslSeqRows* seqs, int n_seqs, int T, int rows) {
     __shared__ int found[READ_ROWS], page_id[READ_ROWS], slot[READ_ROWS];
     grid_dependents_go();
     grid_dependency_wait();
-    const int t0 = (int) blockIdx.x * READ_ROWS;
-    for (int i = 0; i < READ_ROWS; ++i) {
-        const int t = t0 + i, di = t < T ? row_descriptor(seqs, n_seqs, t, &found[i]) : -1;
-        if (threadIdx.x == 0) {
-            int id = -1, in = 0;
-            if (di >= 0) {
-                const NslSeqRows d = seqs[di];
-                const long long pos = (long long) d.pos + (t - d.row);
-                if (pos >= 0 && pos / p.page < p.max_pages) { id = page_of(p, d.seq, (int) (pos / p.page)); in = (int) (pos % p.page); }
-            }
-            page_id[i] = id;
-            slot[i] = in;
+    const int t0 = (int) blockIdx.x * rows, n = min(rows, T - t0);
+    row_descriptors(seqs, n_seqs, t0, n, found);
+    if ((int) threadIdx.x < n) {
+        const int di = found[threadIdx.x];
+        int id = -1, in = 0;
+        if (di >= 0) {
+            const NslSeqRows d = seqs[di];
+            const long long pos = (long long) d.pos + (t0 + (int) threadIdx.x - d.row);
+            if (pos >= 0 && pos / p.page < p.max_pages) { id = page_of(p, d.seq, (int) (pos / p.page)); in = (int) (pos % p.page); }
         }
+        page_id[threadIdx.x] = id;
+        slot[threadIdx.x] = in;
     }
     __syncthreads();
     const int groups = p.hd / 16, per_row = 2 * p.n_kv * groups;
-    for (int i = threadIdx.x; i < READ_ROWS * per_row; i += READ_THREADS) {
+#pragma unroll 2
+    for (int i = threadIdx.x; i < n * per_row; i += READ_THREADS) {
         const int row = i / per_row, g = i % groups, h = i % per_row / groups % p.n_kv, is_v = i % per_row / groups / p.n_kv;
         if (page_id[row] < 0) continue;
         const size_t page_at = ((size_t) layer * p.n_pages + page_id[row]) * p.n_kv + h;
@@ -281,6 +283,15 @@ __device__ int block_scan(int v, int* total) {
 __device__ __forceinline__ int pages_for(int len, int page) { return len / page + (len % page != 0); }
 __device__ __forceinline__ bool seq_ok(const NslPages& p, int seq) { return seq >= 0 && seq < p.n_seq; }
 
+// How many entries before this thread's have the same key (keys >= 0; all[] holds every thread's): a warp's own by a match, those of
+// earlier warps one by one.  Called by whole warps.
+__device__ __forceinline__ int same_before(const int* all, int key) {
+    const uint32_t lower = (1u << (threadIdx.x & 31)) - 1u;
+    int n = __popc(__match_any_sync(0xFFFFFFFFu, key) & lower);
+    for (int j = 0; key >= 0 && j < (int) (threadIdx.x & ~31u); ++j) n += all[j] == key;
+    return n;
+}
+
 __global__ void __launch_bounds__(MAN_THREADS) extend_kernel(NslPages p, const NslPagesLen* reqs, int n, int32_t* got) {
     __shared__ int seq_s[MAN_THREADS], page_s[MAN_THREADS], start_s[MAN_THREADS], have_s[MAN_THREADS], end_s[MAN_THREADS];
     grid_dependents_go();
@@ -291,8 +302,7 @@ __global__ void __launch_bounds__(MAN_THREADS) extend_kernel(NslPages p, const N
     bool fits = i < n && seq_ok(p, seq);
     seq_s[i] = fits ? seq : -1;
     __syncthreads();
-    for (int j = 0; fits && j < i; ++j)
-        if (seq_s[j] == seq) fits = false;      // named before
+    if (same_before(seq_s, fits ? seq : -1) && fits) fits = false;      // named before
     int have = 0, need = 0, last_id = -1;
     if (fits) {
         old = p.len[seq];
@@ -307,15 +317,9 @@ __global__ void __launch_bounds__(MAN_THREADS) extend_kernel(NslPages p, const N
     }
     page_s[i] = fits ? last_id : -1;
     __syncthreads();
-    bool copy = false;
-    if (fits && last_id >= 0) {
-        const int users = p.ref[last_id];
-        if (users > 1) {
-            int before = 0;      // requests that give the page up before this one
-            for (int j = 0; j < i; ++j) before += page_s[j] == last_id;
-            copy = users - before > 1;
-        }
-    }
+    const int users = fits && last_id >= 0 ? p.ref[last_id] : 0;
+    const int given_up = same_before(page_s, page_s[i]);      // requests that give the page up before this one
+    const bool copy = users > 1 && users - given_up > 1;
     const int want = fits ? min(need - have + copy, p.n_pages + 1) : 0;      // (n_pages <= 2^20: the sum stays in 32 bits)
     int total, n_free = 0;
     const int start = block_scan(want, &total);
@@ -373,8 +377,7 @@ __global__ void __launch_bounds__(MAN_THREADS) fork_kernel(NslPages p, const Nsl
     }
     dst_s[i] = on ? dst : -1;
     __syncthreads();
-    for (int j = 0; on && j < i; ++j)
-        if (dst_s[j] == dst) on = false;
+    if (same_before(dst_s, on ? dst : -1) && on) on = false;
     if (on) {
         on = p.len[dst] == 0;
         len = max(min(len, p.len[src]), 0);
@@ -557,11 +560,15 @@ void nsl_pages_append(cudaStream_t s, const NslPages* p, int layer, NslRope r, i
     if ((long long) T * p->n_kv > 1 << 29) { set_error("nsl_pages_append: %d rows of %d heads in one call", T, p->n_kv); return; }
     const long long most = (long long) T / p->page + 2ll * (n_seqs < T ? n_seqs : T);      // sum of (rows - 1) / page + 2
     a.units = (int) (most < T ? most : T);
+    // heads of a block: the keys' angles are made once for all of them, so as many as leave four blocks an SM; rows of queries likewise
     a.heads_each = 1;
-    a.head_split = p->n_kv;
+    while (a.heads_each * 2 <= p->n_kv && (long long) a.units * 2 * (p->n_kv / (a.heads_each * 2)) >= 4ll * sm_count()) a.heads_each *= 2;
+    a.head_split = (p->n_kv + a.heads_each - 1) / a.heads_each;
     a.kv_blocks = a.units * 2 * a.head_split;
-    const int q_blocks = n_head ? (T + APPEND_Q_ROWS - 1) / APPEND_Q_ROWS : 0;
-    const int rows = p->page > APPEND_Q_ROWS ? p->page : APPEND_Q_ROWS;
+    a.q_rows = 1;
+    while (a.q_rows < APPEND_Q_ROWS && T / (a.q_rows * 2) >= 4 * sm_count()) a.q_rows *= 2;
+    const int q_blocks = n_head ? (T + a.q_rows - 1) / a.q_rows : 0;
+    const int rows = p->page > a.q_rows ? p->page : a.q_rows;
     const size_t smem = sizeof(float2) * (size_t) (r.rot / 2) * rows;
     const unsigned blocks = (unsigned) (a.kv_blocks + q_blocks);
     if (type == NSL_F32) launch_append<NSL_F32>(s, a, blocks, smem);
@@ -578,10 +585,12 @@ void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void
         return;
     }
     FollowScope follow;
-    const dim3 grid((unsigned) ((T + READ_ROWS - 1) / READ_ROWS));
-    if (type == NSL_F32) launch(read_kernel<NSL_F32>, grid, READ_THREADS, 0, s, *p, layer, ko, ko_stride, vo, vo_stride, seqs, n_seqs, T);
-    else if (type == NSL_BF16) launch(read_kernel<NSL_BF16>, grid, READ_THREADS, 0, s, *p, layer, ko, ko_stride, vo, vo_stride, seqs, n_seqs, T);
-    else launch(read_kernel<NSL_F32_BF16>, grid, READ_THREADS, 0, s, *p, layer, ko, ko_stride, vo, vo_stride, seqs, n_seqs, T);
+    int rows = 1;      // as many as leave eight blocks an SM
+    while (rows < READ_ROWS && T / (rows * 2) >= 8 * sm_count()) rows *= 2;
+    const dim3 grid((unsigned) ((T + rows - 1) / rows));
+    if (type == NSL_F32) launch(read_kernel<NSL_F32>, grid, READ_THREADS, 0, s, *p, layer, ko, ko_stride, vo, vo_stride, seqs, n_seqs, T, rows);
+    else if (type == NSL_BF16) launch(read_kernel<NSL_BF16>, grid, READ_THREADS, 0, s, *p, layer, ko, ko_stride, vo, vo_stride, seqs, n_seqs, T, rows);
+    else launch(read_kernel<NSL_F32_BF16>, grid, READ_THREADS, 0, s, *p, layer, ko, ko_stride, vo, vo_stride, seqs, n_seqs, T, rows);
     count_launch();
 }
 

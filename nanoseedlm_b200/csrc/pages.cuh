@@ -93,17 +93,15 @@ __device__ __forceinline__ int page_of(const NslPages& p, int seq, int j) {
     const int id = p.table[(size_t) seq * p.max_pages + j];
     return id >= 0 && id < p.n_pages ? id : -1;
 }
-// Of row t: the descriptor that names it, -1 where none does.  All threads of a block call it; `found` is shared memory.
-__device__ __forceinline__ int row_descriptor(const NslSeqRows* seqs, int n_seqs, int t, int* found) {
-    __syncthreads();
-    if (threadIdx.x == 0) *found = -1;
+// Of rows t0 .. t0 + n - 1: the descriptors that name them, -1 where none does, in found (shared memory).  All threads of a block call it.
+__device__ __forceinline__ void row_descriptors(const NslSeqRows* seqs, int n_seqs, int t0, int n, int* found) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) found[i] = -1;
     __syncthreads();
     for (int i = threadIdx.x; i < n_seqs; i += blockDim.x) {
         const NslSeqRows d = seqs[i];
-        if (t >= d.row && t - d.row < d.rows) *found = i;
+        for (int r = max(d.row - t0, 0); r < n && t0 + r - d.row < d.rows; ++r) found[r] = i;
     }
     __syncthreads();
-    return *found;
 }
 #endif
 

@@ -272,7 +272,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     grid_dependents_go();
-    pattn_warm(a);
     grid_dependency_wait();
     // the step's units and the descriptor that this block's first lies in: a warp a descriptor, a lane a column tile
     int* const of_seq = (int*) (smem + F::OFF_TILES);
