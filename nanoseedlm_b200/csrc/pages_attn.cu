@@ -3,9 +3,9 @@
 
 namespace nsl {
 
-// An item's states joined.  Block (b, y): the item that block b of the first pass leaves unfinished, some of its columns.  Up to
-// MERGE_FEW states: a warp a column, everything requested before anything is used; more: four warps a column, every fourth state
-// each.  Bound: latency (a prompt's call of 148 unfinished items of 256 columns moves 80 MB through L2).
+// The states of an unfinished item of the few-row kernel joined.  Block (b, y): the item that block b of the first pass leaves
+// unfinished, some of its columns.  Up to MERGE_FEW states: a warp a column, everything requested before anything is used; more:
+// four warps a column, every fourth state each.  Bound: latency.
 constexpr int MERGE_THREADS = 256, MERGE_WARPS = MERGE_THREADS / 32, MERGE_EACH = 4, MERGE_FEW = 8;
 
 template <int HD>
@@ -94,9 +94,8 @@ __global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a,
 }
 
 void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks, int most_cols) {
-    const int cols = (a.n_head / a.p.n_kv) * (a.max_rows < a.T ? a.max_rows : a.T);      // (checked to fit before the first pass)
-    const int some = cols < most_cols ? cols : most_cols;
-    const dim3 grid((unsigned) blocks, (unsigned) (some <= 64 ? (some + 1) / 2 : 32));
+    const int cols = (a.n_head / a.p.n_kv) * (a.max_rows < a.T ? a.max_rows : a.T), some = cols < most_cols ? cols : most_cols;
+    const dim3 grid((unsigned) blocks, (unsigned) (some + 1) / 2);
     if (a.p.hd == 128) launch(pattn_merge_kernel<128>, grid, MERGE_THREADS, 0, s, a, most_cols);
     else launch(pattn_merge_kernel<64>, grid, MERGE_THREADS, 0, s, a, most_cols);
 }

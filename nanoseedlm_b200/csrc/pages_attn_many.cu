@@ -2,7 +2,7 @@
 //
 // An item is 256 columns ((row, query head) pairs of a KV head) of a sequence as two tiles of 128; a unit is 64 keys of an item.
 // The step's units are dealt evenly to the blocks, one an SM, in order; a run that ends inside an item leaves its state for the
-// merge kernel.  Per unit and tile:
+// join kernel.  Per unit and tile:
 //   S [128][64]  = Q [128][hd] . K^T      A = queries (f16; the first tile's in tensor memory, the second's in shared memory), B = keys [64][hd]
 //   O [128][hd] += W [128][64] . V        A = weights (f16, tensor memory), B = values as [hd][64]
 // Warps: 4 + 4 take the softmax of the two tiles (a thread a column: its row of S is in its tensor memory lane), 4 expand the
@@ -215,8 +215,8 @@ static __device__ __noinline__ float many_query(const PagesAttn& a, size_t at, b
     return fabsf(a.scale) * 1.4426950408889634f * by;
 }
 
-// A column's O (and, second: the other tile's, 128 columns on) out of tensor memory, times by and by1: to a state (part), or to the
-// results.  By whole warps.
+// A column's O (and, second: the other tile's, 128 columns on) out of tensor memory, times by and by1: to a state (part: columns side by
+// side, as its lanes are), or to the results.  By whole warps.
 template <int HD>
 static __device__ __noinline__ void many_results(const PagesAttn& a, uint32_t to, bool second, float by, float by1, bool valid, float* part, size_t at) {
 #pragma unroll 1
@@ -233,8 +233,10 @@ static __device__ __noinline__ void many_results(const PagesAttn& a, uint32_t to
             if (second) z = fmaf(__uint_as_float(v1[r]), by1, z);
             o[r < 8 ? 2 * r : 2 * (r - 8) + 1] = z;
         }
-        if (part) { store8<NSL_F32>(part, d, o); store8<NSL_F32>(part, d + 8, o + 8); }
-        else if (a.o_type == NSL_BF16) { store8<NSL_BF16>(a.o, at + d, o); store8<NSL_BF16>(a.o, at + d + 8, o + 8); }
+        if (part) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) part[(d + e) * MANY_COLS] = o[e];
+        } else if (a.o_type == NSL_BF16) { store8<NSL_BF16>(a.o, at + d, o); store8<NSL_BF16>(a.o, at + d + 8, o + 8); }
         else { store8<NSL_F32_BF16>(a.o, at + d, o); store8<NSL_F32_BF16>(a.o, at + d + 8, o + 8); }
     }
 }
@@ -476,9 +478,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
             if (warp_valid && !(shared && t)) {
                 const bool second = shared && it.x1 - it.x0 > 1;      // (an O that nothing was added to holds anything)
                 if (parts == 1) { const float fac = pattn_factor(m, l, mo); by *= fac; by1 *= fac; }
-                float* const part = a.part + ((size_t) (2 * blockIdx.x + ((int) blockIdx.x == b0)) * MANY_COLS + c0 + c) * STATE;
+                float* const part = a.part + (size_t) (2 * blockIdx.x + ((int) blockIdx.x == b0)) * MANY_COLS * STATE + c0 + c;
                 many_results<HD>(a, to, second, by, by1, valid, parts > 1 ? part : NULL, (size_t) row * a.o_stride + (size_t) head * HD);
-                if (parts > 1 && valid) *(float4*) (part + HD) = make_float4(m, l, mo, 0.0f);
+                if (parts > 1 && valid) { part[HD * MANY_COLS] = m; part[(HD + 1) * MANY_COLS] = l; part[(HD + 2) * MANY_COLS] = mo; }
             }
             if (shared) {      // the second tile's O has been read
                 tm_before();
@@ -641,12 +643,76 @@ int pattn_many_status() {
     return v;
 }
 
+// The states of an unfinished item joined.  Block (b, y): the item that block b leaves unfinished, columns 32 y .. 32 y + 31; a lane a
+// column, a warp an eighth of the dims, so the states are read as they were written, 128 bytes a warp; the results are turned
+// round in shared memory.
+constexpr int JOIN_THREADS = 256, JOIN_COLS = 32, JOIN_EACH = 4;
+template <int HD>
+__global__ void __launch_bounds__(JOIN_THREADS) pattn_join_kernel(const __grid_constant__ PagesAttn a) {
+    constexpr int STATE = PATTN_STATE<HD>, DIMS = HD / (JOIN_THREADS / 32);
+    __shared__ float turn[JOIN_COLS][HD + 1];
+    grid_dependents_go();
+    grid_dependency_wait();
+    const int4 rec = a.rec[blockIdx.x];
+    const int parts = rec.x & 0xFFFF, kvh = rec.x >> 16, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = (int) blockIdx.y * JOIN_COLS, group = a.n_head / a.p.n_kv;
+    if (parts == 0 || c0 >= rec.w) return;
+    auto state = [&](int i) { return a.part + (size_t) (2 * ((int) blockIdx.x + i) + (i == 0)) * MANY_COLS * STATE + c0 + lane; };      // (columns behind the last: never written, not used)
+    float m = -INFINITY, mo = -INFINITY, l = 0.0f, o[DIMS];
+#pragma unroll
+    for (int e = 0; e < DIMS; ++e) o[e] = 0.0f;
+    for (int i0 = 0; i0 < parts; i0 += JOIN_EACH) {      // some states at a time, everything of them requested at once
+        float sm[JOIN_EACH], sl[JOIN_EACH], so[JOIN_EACH], v[JOIN_EACH][DIMS];
+#pragma unroll
+        for (int i = 0; i < JOIN_EACH; ++i) {
+            sm[i] = so[i] = -INFINITY;
+            sl[i] = 0.0f;
+            if (i0 + i >= parts) continue;
+            const float* p = state(i0 + i);
+            sm[i] = p[HD * MANY_COLS];
+            sl[i] = p[(HD + 1) * MANY_COLS];
+            so[i] = p[(HD + 2) * MANY_COLS];
+#pragma unroll
+            for (int e = 0; e < DIMS; ++e) v[i][e] = p[(warp * DIMS + e) * MANY_COLS];
+        }
+        const float m0 = m, mo0 = mo;
+#pragma unroll
+        for (int i = 0; i < JOIN_EACH; ++i) { m = fmaxf(m, sm[i]); mo = fmaxf(mo, so[i]); }
+        const float ms = m == -INFINITY ? 0.0f : m, mos = mo == -INFINITY ? 0.0f : mo, by = pa_ex2(mo0 - mos);
+        l *= pa_ex2(m0 - ms);
+#pragma unroll
+        for (int e = 0; e < DIMS; ++e) o[e] *= by;
+#pragma unroll
+        for (int i = 0; i < JOIN_EACH; ++i)
+            if (i0 + i < parts) {
+                const float w = pa_ex2(so[i] - mos);
+                l = fmaf(sl[i], pa_ex2(sm[i] - ms), l);
+#pragma unroll
+                for (int e = 0; e < DIMS; ++e) o[e] = fmaf(v[i][e], w, o[e]);
+            }
+    }
+    const float f = pattn_factor(m, l, mo);
+#pragma unroll
+    for (int e = 0; e < DIMS; ++e) turn[lane][warp * DIMS + e] = o[e] * f;
+    __syncthreads();
+    constexpr int EIGHTS = HD / 8;
+    for (int i = threadIdx.x; i < JOIN_COLS * EIGHTS; i += JOIN_THREADS) {
+        const int cl = i / EIGHTS, d = 8 * (i % EIGHTS), c = rec.z + c0 + cl;
+        if (c0 + cl >= rec.w) break;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = turn[cl][d + e];
+        const size_t at = (size_t) (rec.y + c / group) * a.o_stride + (size_t) (kvh * group + c % group) * HD + d;
+        if (a.o_type == NSL_BF16) store8<NSL_BF16>(a.o, at, v); else store8<NSL_F32_BF16>(a.o, at, v);
+    }
+}
+
 template <int HD, bool WIDE>
 static void launch_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
     const unsigned blocks = (unsigned) sm_count();
     cudaFuncSetAttribute(pattn_many_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<HD>::SMEM);
     launch(pattn_many_kernel<HD, WIDE>, blocks, MANY_THREADS, Many<HD>::SMEM, s, a, tk, tv);
-    launch_pattn_merge(s, a, (int) blocks, MANY_COLS);
+    const int cols = (a.n_head / a.p.n_kv) * (a.max_rows < a.T ? a.max_rows : a.T);
+    launch(pattn_join_kernel<HD>, dim3(blocks, (unsigned) (cols < MANY_COLS ? (cols + JOIN_COLS - 1) / JOIN_COLS : MANY_COLS / JOIN_COLS)), JOIN_THREADS, 0, s, a);
     count_launch(2);
 }
 
