@@ -168,47 +168,55 @@ __device__ __forceinline__ void many_sts(uint32_t at, uint32_t a, uint32_t b, ui
 }
 
 // A column's query divided by its power of two, as f16 to tensor memory (tq) or, tq = 0, to its row of the shared panels of 64 dims
-// (at sq; sx: the row's swizzle).  -> |scale| log2 e times that power.  Requested whole where it fits the registers (bf16), for its
-// maximum first and then again otherwise.  Out of line, as its registers would be taken from the softmax.
+// (at sq; sx: the row's swizzle).  -> |scale| log2 e times that power.  Out of line, as its registers would be taken from the
+// softmax, and in short loops: code that runs once an item is fetched anew each time, and unrolled it took 10 us an item.
 template <int HD>
 static __device__ __noinline__ float many_query(const PagesAttn& a, size_t at, bool valid, uint32_t tq, uint32_t sq, uint32_t sx) {
-    uint4 raw[HD / 8];
+    const bool packed = a.q_type == NSL_BF16;
     float top = 0.0f;
-    if (a.q_type == NSL_BF16) {
+    if (valid) {
+        if (packed) {
+            uint32_t most = 0;      // magnitudes of bf16 values order as integers
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 64)
 #pragma unroll
-        for (int j = 0; j < HD / 8; ++j) raw[j] = valid ? *(const uint4*) ((const uint16_t*) a.q + at + 8 * j) : make_uint4(0u, 0u, 0u, 0u);
+                for (int j = 0; j < 8; ++j) {
+                    const uint4 u = *(const uint4*) ((const uint16_t*) a.q + at + d + 8 * j);
+                    most = __vmaxu2(__vmaxu2(most, u.x & 0x7FFF7FFFu), __vmaxu2(u.y & 0x7FFF7FFFu, __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu)));
+                }
+            top = __uint_as_float(max(most << 16, most & 0xFFFF0000u));
+        } else {
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 32)
 #pragma unroll
-        for (int j = 0; j < HD / 8; ++j) {
-            float v[8];
-            eight_of(raw[j], v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
-        }
-    } else if (valid) {
-#pragma unroll 16
-        for (int d = 0; d < HD; d += 4) {
-            const float4 v = *(const float4*) ((const float*) a.q + at + d);
-            top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                for (int j = 0; j < 8; ++j) {
+                    const float4 v = *(const float4*) ((const float*) a.q + at + d + 4 * j);
+                    top = max3(max3(top, fabsf(v.x), fabsf(v.y)), fabsf(v.z), fabsf(v.w));
+                }
         }
     }
     const float by = pa_pow2_of(top), inv = copysignf(1.0f / by, a.scale);      // the scale's sign goes with the query: maxima are then of scores
-#pragma unroll
+#pragma unroll 1
     for (int d = 0; d < HD; d += 32) {
         uint32_t w[16];
+        float v[32];
+        if (!valid) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float v[8];
-            if (a.q_type == NSL_BF16) eight_of(raw[d / 8 + j], v);
-            else if (valid) load8<NSL_F32>(a.q, at + d + 8 * j, v);
-            else {
+            for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+        } else if (packed) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-            }
+            for (int j = 0; j < 4; ++j) load8<NSL_BF16>(a.q, at + d + 8 * j, v + 8 * j);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[4 * j + e] = pa_f16x2(v[2 * e] * inv, v[2 * e + 1] * inv);
-            if (!tq) many_sts(sq + (d >> 6) * (MANY_TILE * 128) + (((uint32_t) ((d & 63) / 8 + j) ^ sx) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            for (int j = 0; j < 4; ++j) load8<NSL_F32>(a.q, at + d + 8 * j, v + 8 * j);
         }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pa_f16x2(v[2 * e] * inv, v[2 * e + 1] * inv);
         if (tq) tm_st16(tq + d / 2, w);
+        else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) many_sts(sq + (d >> 6) * (MANY_TILE * 128) + (((uint32_t) ((d & 63) / 8 + j) ^ sx) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        }
     }
     if (tq) tm_wait_st();
     else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
