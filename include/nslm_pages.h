@@ -81,16 +81,21 @@ void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void
 
 /* Attention of each sequence's rows over its pages: the row at position P attends positions max(0, P - window + 1) .. P
  * (window <= 0: from 0) of its sequence, query head h over KV head h / (n_head / n_kv).  o = softmax(scale q.k) v, rounded to
- * bf16 (o_type NSL_BF16 or NSL_F32_BF16).  Positions without a page are left out; a row that nothing is left for gives zeros.
+ * bf16 (o_type NSL_BF16 or NSL_F32_BF16; o does not overlap q).  Positions without a page are left out, and so is what lies in a
+ * page behind the row's position, whatever it holds; a row that nothing is left for gives zeros.  Scales are not negative.  Here a
+ * sequence may appear in several descriptors.
  * Queries take part with 11 significant bits (bf16 values exactly), weights with 11, sums in f32.
  * max_rows: no descriptor has more rows (rows beyond it are left as they are).  work: nsl_pages_attn_work() bytes of device
  * memory, 16-byte aligned, no initial contents; calls that share it run one behind the other, captured ones too.
- * The steps' keys are dealt evenly to the blocks, so a row alone and in a batch may differ in the order of its f32 sums. */
+ * The step's keys are dealt evenly to the blocks, so a row alone and in a batch may differ in the order of its f32 sums; a call
+ * repeated gives the same bits.  n_seqs <= 4096; the 64-key units of a call (all sequences and KV heads) number fewer than 2^31. */
 size_t nsl_pages_attn_work(void);
 void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, const void* q, int q_stride, int n_head, float scale, int window,
                     const NslSeqRows* seqs, int n_seqs, int max_rows, int T, int o_type, void* o, int o_stride, void* work);
-/* 0, or the code of the first bounded device-side wait that ran out in an attention block since the last call (1 a fetch waiting
- * for a free stage, 2 a computing warp waiting for a full one); the rows of such a block are not valid.  Call after synchronising. */
+/* 0, or the code of the first bounded device-side wait that ran out in an attention block since the last call (few rows: 1 a fetch
+ * waiting for a free stage, 2 a computing warp waiting for a full one; many rows: 4 .. 6 the softmax waiting for scores, for
+ * scales or for values added, 7 and 8 the expansion for codes or a free tile, 9 a fetch, 10 .. 13 the issue of products for
+ * queries, tiles, read scores or weights); the results of such a block are not valid.  Call after synchronising. */
 int nsl_pages_attn_status(void);
 
 /* ---- management: device lists, at most NSL_PAGES_LIST entries a call; the calls on a pool run one behind the other -------- */

@@ -52,14 +52,19 @@ __device__ __forceinline__ void store8(void* base, size_t at, const float* x) {
     store8<NSL_F32>(base, at, y);
 }
 
-// (factor cos a, factor sin a) for a = pos * inv.  The product of an int32 and an f32 has at most 55 significant bits and is
-// reduced to half a turn in f64: an f32 product would be off by pos * inv * 2^-24, 0.06 at a million positions.
+// (factor cos a, factor sin a) for a = pos * inv, each rounded to f32 once.  The product of an int32 and an f32 has at most 55
+// significant bits; an f32 product would be off by pos * inv * 2^-24, 0.06 at a million positions.  In f64: reduced by the nearest
+// multiple of pi / 2 (in two parts: exact to 1e-16 for every position), then the Taylor sums of sine and cosine on [-pi/4, pi/4]
+// (first terms left out: r^13 / 13!, r^12 / 12!, below 2e-10), a quarter turn at a time.  Keys that lie at the border between two
+// codes then fall as the formula has them.
 __device__ __forceinline__ float2 rope_angle(int pos, float inv, float factor) {
-    double a = (double) pos * (double) inv;
-    a = fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
-    float sn, cs;
-    sincosf((float) a, &sn, &cs);
-    return make_float2(cs * factor, sn * factor);
+    const double a = (double) pos * (double) inv, k = rint(a * 0.63661977236758134);
+    const double r = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, a)), z = r * r;
+    const double sn = fma(r * z, fma(z, fma(z, fma(z, fma(z, -1.0 / 39916800.0, 1.0 / 362880.0), -1.0 / 5040.0), 1.0 / 120.0), -1.0 / 6.0), r);
+    const double cs = fma(z, fma(z, fma(z, fma(z, fma(z, -1.0 / 3628800.0, 1.0 / 40320.0), -1.0 / 720.0), 1.0 / 24.0), -0.5), 1.0);
+    const int q = (int) ((long long) k & 3);
+    const double c = q & 1 ? sn : cs, s = q & 1 ? cs : sn;
+    return make_float2((float) ((q == 1 || q == 2 ? -c : c) * factor), (float) ((q >= 2 ? -s : s) * factor));
 }
 // Groups of 16 of a head's values, read as two runs of 8: group g < rot / 16 is rotated by the pairs 8 g .. 8 g + 7, the others
 // are dims 16 g .. 16 g + 15 as they are.
@@ -68,21 +73,21 @@ __device__ __forceinline__ void rope_runs(const NslRope& r, int g, int* a, int* 
     *a = half ? 8 * g : 16 * g;
     *b = half ? 8 * g + r.rot / 2 : 16 * g + 8;
 }
-// x: the two runs; cs: (cos, sin) of the group's 8 pairs.
+// x: the two runs; cs: (cos, sin) of the group's 8 pairs.  Every product and sum is rounded to f32 by itself, as the formula reads.
 __device__ __forceinline__ void rope_turn(int layout, float* x, const float2* cs) {
     if (layout == NSL_ROPE_HALF) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float u = x[i], w = x[i + 8];
-            x[i] = u * cs[i].x - w * cs[i].y;
-            x[i + 8] = w * cs[i].x + u * cs[i].y;
+            x[i] = __fsub_rn(__fmul_rn(u, cs[i].x), __fmul_rn(w, cs[i].y));
+            x[i + 8] = __fadd_rn(__fmul_rn(w, cs[i].x), __fmul_rn(u, cs[i].y));
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float u = x[2 * i], w = x[2 * i + 1];
-            x[2 * i] = u * cs[i].x - w * cs[i].y;
-            x[2 * i + 1] = w * cs[i].x + u * cs[i].y;
+            x[2 * i] = __fsub_rn(__fmul_rn(u, cs[i].x), __fmul_rn(w, cs[i].y));
+            x[2 * i + 1] = __fadd_rn(__fmul_rn(w, cs[i].x), __fmul_rn(u, cs[i].y));
         }
     }
 }

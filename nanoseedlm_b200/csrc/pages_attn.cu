@@ -22,7 +22,7 @@ __device__ __forceinline__ void merge_add(float4& o, const float4& v, float w) {
 __device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.0f : m; }
 
 template <int HD>
-__global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a, int most_cols) {
+__global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a) {
     constexpr int STATE = PATTN_STATE<HD>;
     __shared__ float4 sum[MERGE_WARPS][32];
     __shared__ float stat[MERGE_WARPS][3];
@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a,
     const int4 rec = a.rec[blockIdx.x];
     const int parts = rec.x & 0xFFFF, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (parts == 0) return;
-    auto state = [&](int i, int col) { return a.part + ((size_t) (2 * ((int) blockIdx.x + i) + (i == 0)) * most_cols + col) * STATE; };
+    auto state = [&](int i, int col) { return a.part + ((size_t) (2 * ((int) blockIdx.x + i) + (i == 0)) * PATTN_FEW + col) * STATE; };
     if (parts <= MERGE_FEW) {
         for (int col = (int) blockIdx.y * MERGE_WARPS + warp; col < rec.w; col += (int) gridDim.y * MERGE_WARPS) {
             float4 v[MERGE_FEW], st[MERGE_FEW];
@@ -93,11 +93,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) pattn_merge_kernel(PagesAttn a,
     }
 }
 
-void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks, int most_cols) {
-    const int cols = (a.n_head / a.p.n_kv) * (a.max_rows < a.T ? a.max_rows : a.T), some = cols < most_cols ? cols : most_cols;
-    const dim3 grid((unsigned) blocks, (unsigned) (some + 1) / 2);
-    if (a.p.hd == 128) launch(pattn_merge_kernel<128>, grid, MERGE_THREADS, 0, s, a, most_cols);
-    else launch(pattn_merge_kernel<64>, grid, MERGE_THREADS, 0, s, a, most_cols);
+void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks) {
+    const dim3 grid((unsigned) blocks, (unsigned) ((a.n_head / a.p.n_kv) * a.max_rows + 1) / 2);      // (at most PATTN_FEW columns)
+    if (a.p.hd == 128) launch(pattn_merge_kernel<128>, grid, MERGE_THREADS, 0, s, a);
+    else launch(pattn_merge_kernel<64>, grid, MERGE_THREADS, 0, s, a);
 }
 
 // Encoded at every call: a map is 128 bytes of the launch's arguments, and a pool's buffers are the caller's.
@@ -149,10 +148,11 @@ void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, co
     a.rec = (int4*) work;
     a.part = (float*) ((char*) work + 16 * (size_t) pattn_blocks());
     a.scale = scale; a.q_type = q_type; a.q_stride = q_stride; a.o_type = o_type; a.o_stride = o_stride;
-    a.n_head = n_head; a.layer = layer; a.window = window; a.n_seqs = n_seqs; a.max_rows = max_rows; a.T = T;
-    // One of the two for all sequences of a call: beside sequences of many rows those of few ones cost less in the wide kernel's blocks than
-    // in two more launches (32 decode rows of 4096 keys beside a chunk: see pages_attn_many.cu).
-    if ((long long) (n_head / p->n_kv) * (max_rows < T ? max_rows : T) <= PATTN_FEW) launch_pattn_few(s, a, tk, tv);
+    a.n_head = n_head; a.layer = layer; a.window = window; a.n_seqs = n_seqs; a.max_rows = max_rows < T ? max_rows : T; a.T = T;
+    // One of the two for all sequences of a call.  The few-row kernel reads the keys for 8 columns at a time, the wide one makes a tile of 128
+    // whatever it holds: 32 rows of 4096 keys with 8 heads a KV head 21 against 49 us, with 16 columns (two passes' registers) 57 against
+    // 51, 8 rows with 16 heads 32 against 29.  Beside a prompt's rows decode rows cost less in the wide kernel's blocks than two more launches.
+    if ((long long) (n_head / p->n_kv) * a.max_rows <= PATTN_FEW) launch_pattn_few(s, a, tk, tv);
     else launch_pattn_many(s, a, tk, tv);
 }
 

@@ -21,13 +21,13 @@ struct PagesAttn {
 
 // Blocks of a launch at most: two an SM (their number fits a record's 16 bits).
 inline int pattn_blocks() { return 2 * sm_count(); }
-constexpr int PATTN_FEW = 16, PATTN_MANY = 256;      // columns of an item
+constexpr int PATTN_FEW = 8, PATTN_MANY = 256;      // columns of an item
 template <int HD>
 constexpr int PATTN_STATE = HD + 4;      // floats of a column's state: O [HD], m, l, mo, one unused
 void launch_pattn_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv);
 int pattn_few_status();
 int pattn_many_status();
-void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks, int most_cols);
+void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks);
 
 bool pattn_map(CUtensorMap* tm, const NslPages& p, const int8_t* codes);      // rows of hd codes, boxes of min(page, 64) rows, swizzled
 void launch_pattn_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv);
@@ -111,7 +111,7 @@ __device__ __forceinline__ float pa_pow2_of(float x) {
 __device__ __forceinline__ void pattn_warm(const PagesAttn& a) {
     const size_t scales = (size_t) a.layer * a.p.n_pages * a.p.n_kv, scale_lines = ((size_t) a.p.n_pages * a.p.n_kv * 4 + 127) / 128;
     const char* const from[5] = {(const char*) a.seqs, (const char*) a.p.table, (const char*) (a.p.ks + scales), (const char*) (a.p.vs + scales), (const char*) a.q};
-    const size_t lines[5] = {((size_t) a.n_seqs * sizeof(NslSeqRows) + 127) / 128, ((size_t) a.p.n_seq * a.p.max_pages * 4 + 127) / 128, scale_lines, scale_lines, ((size_t) a.T * a.q_stride * (a.q_type == NSL_BF16 ? 2 : 4) + 127) / 128};
+    const size_t lines[5] = {((size_t) a.n_seqs * sizeof(NslSeqRows) + 127) / 128, ((size_t) a.p.n_seq * a.p.max_pages * 4 + 127) / 128, scale_lines, scale_lines, (((size_t) (a.T - 1) * a.q_stride + (size_t) a.n_head * a.p.hd) * (a.q_type == NSL_BF16 ? 2 : 4) + 127) / 128};
     const size_t at = (size_t) blockIdx.x * blockDim.x + threadIdx.x;      // one line of each array a thread: 9 MB a launch
 #pragma unroll
     for (int i = 0; i < 5; ++i)

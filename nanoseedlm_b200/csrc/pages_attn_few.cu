@@ -1,4 +1,4 @@
-// Attention over the paged cache for sequences with few rows (decode, verify): at most 16 columns, a column being one (row, query
+// Attention over the paged cache for sequences with few rows (decode, verify): at most 8 columns, a column being one (row, query
 // head) of a KV head.
 //
 // Bound: HBM, 2 hd + 8 / page bytes a key and KV head.  The step's keys are cut into units of 64 of one (sequence, KV head) and
@@ -19,9 +19,9 @@ namespace nsl {
 
 constexpr int FEW_KEYS = 64, FEW_WARPS = 4, FEW_THREADS = 32 * (FEW_WARPS + 1);
 
-template <int HD, int NT>
+template <int HD>
 struct Few {
-    static constexpr int CT = 8 * NT;                    // columns
+    static constexpr int CT = PATTN_FEW;                 // columns
     static constexpr int TILE = FEW_KEYS * HD;           // bytes of a unit's keys, or values
     static constexpr int STAGES = HD == 128 ? 5 : 9;
     static constexpr int STATE = PATTN_STATE<HD>;        // floats of a column's partial state: O, then m, l, mo
@@ -110,9 +110,9 @@ __device__ __forceinline__ void few_weights(const float* p, int c, float* cw, fl
     of_all[3 * c] = m; of_all[3 * c + 1] = l; of_all[3 * c + 2] = mo;
 }
 
-template <int HD, int NT>
+template <int HD>
 __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
-    using F = Few<HD, NT>;
+    using F = Few<HD>;
     constexpr int CT = F::CT, STATE = F::STATE, STEPS = HD / 16;
     extern __shared__ uint8_t few_raw[];
     uint8_t* const smem = (uint8_t*) (((uintptr_t) few_raw + 1023) & ~(uintptr_t) 1023);
@@ -228,60 +228,52 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
     while (walk.next(a, group, x, xe, &it)) {
         const int cols = it.sp.rows * group;
         // the queries as B fragments: column r0 of a tile, dims 16 j + 4 q4 ..; a column divided by its power of two
-        uint32_t qb[NT][STEPS][2];
-        float f[NT][2];      // of the lane's columns 2 q4, 2 q4 + 1: scale, log2 e and the power of two
-        int hi[NT][2], lo[NT][2];
+        uint32_t qb[STEPS][2];
+        float f[2];      // of the lane's columns 2 q4, 2 q4 + 1: scale, log2 e and the power of two
+        int hi[2], lo[2];
+        const int c = r0;
+        float v[STEPS][4], top = 0.0f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int c = 8 * nt + r0;
-            float v[STEPS][4], top = 0.0f;
-#pragma unroll
-            for (int j = 0; j < STEPS; ++j) {
-                const size_t at = (size_t) (it.sp.row + c / group) * a.q_stride + (size_t) (it.kvh * group + c % group) * HD + 16 * j + 4 * q4;
-                if (c >= cols) v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.0f;
-                else if (a.q_type == NSL_BF16) {
-                    const uint2 u = *(const uint2*) ((const uint16_t*) a.q + at);
-                    v[j][0] = __uint_as_float(u.x << 16); v[j][1] = __uint_as_float(u.x & 0xFFFF0000u); v[j][2] = __uint_as_float(u.y << 16); v[j][3] = __uint_as_float(u.y & 0xFFFF0000u);
-                } else {
-                    const float4 u = *(const float4*) ((const float*) a.q + at);
-                    v[j][0] = u.x; v[j][1] = u.y; v[j][2] = u.z; v[j][3] = u.w;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[j][e]));
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const float by = pa_pow2_of(top), inv = copysignf(1.0f / by, a.scale), fc = fabsf(a.scale) * 1.4426950408889634f * by;
-#pragma unroll
-            for (int j = 0; j < STEPS; ++j) {
-                qb[nt][j][0] = pa_f16x2(v[j][0] * inv, v[j][1] * inv);
-                qb[nt][j][1] = pa_f16x2(v[j][2] * inv, v[j][3] * inv);
+        for (int j = 0; j < STEPS; ++j) {
+            const size_t at = (size_t) (it.sp.row + c / group) * a.q_stride + (size_t) (it.kvh * group + c % group) * HD + 16 * j + 4 * q4;
+            if (c >= cols) v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.0f;
+            else if (a.q_type == NSL_BF16) {
+                const uint2 u = *(const uint2*) ((const uint16_t*) a.q + at);
+                v[j][0] = __uint_as_float(u.x << 16); v[j][1] = __uint_as_float(u.x & 0xFFFF0000u); v[j][2] = __uint_as_float(u.y << 16); v[j][3] = __uint_as_float(u.y & 0xFFFF0000u);
+            } else {
+                const float4 u = *(const float4*) ((const float*) a.q + at);
+                v[j][0] = u.x; v[j][1] = u.y; v[j][2] = u.z; v[j][3] = u.w;
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                f[nt][e] = __shfl_sync(0xFFFFFFFFu, fc, 4 * (2 * q4 + e));
-                const int cc = 8 * nt + 2 * q4 + e, pos = it.sp.pos + cc / group;
-                hi[nt][e] = cc < cols ? pos : -1;
-                lo[nt][e] = a.window > 0 ? pos - a.window + 1 : 0;
-            }
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[j][e]));
         }
-        float m[NT][2], mo[NT][2], l[NT][2], ot[NT][STEPS][4];
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        const float by = pa_pow2_of(top), inv = copysignf(1.0f / by, a.scale), fc = fabsf(a.scale) * 1.4426950408889634f * by;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            m[nt][0] = m[nt][1] = mo[nt][0] = mo[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) ot[nt][i][0] = ot[nt][i][1] = ot[nt][i][2] = ot[nt][i][3] = 0.0f;
+        for (int j = 0; j < STEPS; ++j) {
+            qb[j][0] = pa_f16x2(v[j][0] * inv, v[j][1] * inv);
+            qb[j][1] = pa_f16x2(v[j][2] * inv, v[j][3] * inv);
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            f[e] = __shfl_sync(0xFFFFFFFFu, fc, 4 * (2 * q4 + e));
+            const int cc = 2 * q4 + e, pos = it.sp.pos + cc / group;
+            hi[e] = cc < cols ? pos : -1;
+            lo[e] = a.window > 0 ? pos - a.window + 1 : 0;
+        }
+        float m[2], mo[2], l[2], ot[STEPS][4];
+        m[0] = m[1] = mo[0] = mo[1] = -INFINITY;
+        l[0] = l[1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) ot[i][0] = ot[i][1] = ot[i][2] = ot[i][3] = 0.0f;
         for (x = it.x0; x < it.x1; ++x) {
             wait(full + 8 * stage, round & 1, 2);
             const float4 mt = meta[4 * stage + warp];
             const int key = (it.tile0 + x - it.first) * FEW_KEYS + 16 * warp;
             if (mt.z != 0.0f && key < it.k1 && key + 16 > it.k0) {
                 const uint32_t kt = ring + stage * 2 * F::TILE + l_at;
-                float s[NT][4], s2[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.0f;
+                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // two chains
 #pragma unroll
                 for (int j = 0; j < STEPS; j += 2) {
                     uint32_t c[4];
@@ -290,45 +282,42 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
                     for (int e = 0; e < 4; ++e) c[e] ^= 0x80808080u;
                     const uint32_t a0[4] = {pa_codes<0x4140>(c[0]), pa_codes<0x4140>(c[1]), pa_codes<0x4342>(c[0]), pa_codes<0x4342>(c[1])};
                     const uint32_t a1[4] = {pa_codes<0x4140>(c[2]), pa_codes<0x4140>(c[3]), pa_codes<0x4342>(c[2]), pa_codes<0x4342>(c[3])};
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) { few_mma(s[nt], a0, qb[nt][j]); few_mma(s2[nt], a1, qb[nt][j + 1]); }
+                    few_mma(s, a0, qb[j]);
+                    few_mma(s2, a1, qb[j + 1]);
                 }
-                uint32_t pw[NT][2];
+                uint32_t pw[2];
+                float mx[2];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float mx[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {      // keys key + r0 and key + r0 + 8 of column 2 q4 + e
-                        const float fk = f[nt][e] * mt.x;
-                        const int ka = key + r0, kb = ka + 8;
-                        s[nt][e] = ka <= hi[nt][e] && ka >= lo[nt][e] ? (s[nt][e] + s2[nt][e]) * fk : -INFINITY;
-                        s[nt][2 + e] = kb <= hi[nt][e] && kb >= lo[nt][e] ? (s[nt][2 + e] + s2[nt][2 + e]) * fk : -INFINITY;
-                        mx[e] = fmaxf(s[nt][e], s[nt][2 + e]);
-                    }
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) {
-                        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xFFFFFFFFu, mx[0], o));
-                        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xFFFFFFFFu, mx[1], o));
-                    }
-                    float cor[2], w[4];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float mn = fmaxf(m[nt][e], mx[e]), ms = mn == -INFINITY ? 0.0f : mn;
-                        const float mon = fmaxf(mo[nt][e], mx[e] + mt.y), mos = mon == -INFINITY ? 0.0f : mon;
-                        l[nt][e] = fmaf(l[nt][e], pa_ex2(m[nt][e] - ms), pa_ex2(s[nt][e] - ms) + pa_ex2(s[nt][2 + e] - ms));
-                        cor[e] = pa_ex2(mo[nt][e] - mos);
-                        w[e] = s[nt][e] == -INFINITY ? 0.0f : pa_ex2(s[nt][e] + (mt.y - mos));      // (an infinite scale counts for those who attend its page)
-                        w[2 + e] = s[nt][2 + e] == -INFINITY ? 0.0f : pa_ex2(s[nt][2 + e] + (mt.y - mos));
-                        m[nt][e] = mn;
-                        mo[nt][e] = mon;
-                    }
-                    if (cor[0] != 1.0f || cor[1] != 1.0f) {      // the running maxima rarely move after a run's first steps
-#pragma unroll
-                        for (int i = 0; i < STEPS; ++i) { ot[nt][i][0] *= cor[0]; ot[nt][i][1] *= cor[1]; ot[nt][i][2] *= cor[0]; ot[nt][i][3] *= cor[1]; }
-                    }
-                    pw[nt][0] = few_turn(pa_f16x2(w[0], w[1]));
-                    pw[nt][1] = few_turn(pa_f16x2(w[2], w[3]));
+                for (int e = 0; e < 2; ++e) {      // keys key + r0 and key + r0 + 8 of column 2 q4 + e
+                    const float fk = f[e] * mt.x;
+                    const int ka = key + r0, kb = ka + 8;
+                    s[e] = ka <= hi[e] && ka >= lo[e] ? (s[e] + s2[e]) * fk : -INFINITY;
+                    s[2 + e] = kb <= hi[e] && kb >= lo[e] ? (s[2 + e] + s2[2 + e]) * fk : -INFINITY;
+                    mx[e] = fmaxf(s[e], s[2 + e]);
                 }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xFFFFFFFFu, mx[0], o));
+                    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xFFFFFFFFu, mx[1], o));
+                }
+                float cor[2], w[4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mn = fmaxf(m[e], mx[e]), ms = mn == -INFINITY ? 0.0f : mn;
+                    const float mon = fmaxf(mo[e], mx[e] + mt.y), mos = mon == -INFINITY ? 0.0f : mon;
+                    l[e] = fmaf(l[e], pa_ex2(m[e] - ms), pa_ex2(s[e] - ms) + pa_ex2(s[2 + e] - ms));
+                    cor[e] = pa_ex2(mo[e] - mos);
+                    w[e] = s[e] == -INFINITY ? 0.0f : pa_ex2(s[e] + (mt.y - mos));      // (an infinite scale counts for those who attend its page)
+                    w[2 + e] = s[2 + e] == -INFINITY ? 0.0f : pa_ex2(s[2 + e] + (mt.y - mos));
+                    m[e] = mn;
+                    mo[e] = mon;
+                }
+                if (cor[0] != 1.0f || cor[1] != 1.0f) {      // the running maxima rarely move after a run's first steps
+#pragma unroll
+                    for (int i = 0; i < STEPS; ++i) { ot[i][0] *= cor[0]; ot[i][1] *= cor[1]; ot[i][2] *= cor[0]; ot[i][3] *= cor[1]; }
+                }
+                pw[0] = few_turn(pa_f16x2(w[0], w[1]));
+                pw[1] = few_turn(pa_f16x2(w[2], w[3]));
 #pragma unroll
                 for (int j = 0; j < STEPS; j += 2) {
                     uint32_t c[4];
@@ -338,8 +327,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
                     // row r0 of value tile j: dim 16 j + 2 r0, row r0 + 8: the next
                     const uint32_t a0[4] = {pa_codes<0x4240>(c[0]), pa_codes<0x4341>(c[0]), pa_codes<0x4240>(c[1]), pa_codes<0x4341>(c[1])};
                     const uint32_t a1[4] = {pa_codes<0x4240>(c[2]), pa_codes<0x4341>(c[2]), pa_codes<0x4240>(c[3]), pa_codes<0x4341>(c[3])};
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) { few_mma(ot[nt][j], a0, pw[nt]); few_mma(ot[nt][j + 1], a1, pw[nt]); }
+                    few_mma(ot[j], a0, pw);
+                    few_mma(ot[j + 1], a1, pw);
                 }
             }
             __syncwarp();      // the stage has been read by all lanes
@@ -349,16 +338,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
         // the warps' states side by side, merged into the block's
         few_sync();      // the last item's states have been read
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int o = 4; o < 32; o <<= 1) l[e] += __shfl_xor_sync(0xFFFFFFFFu, l[e], o);
+            float* st = merge + (size_t) (warp * CT + 2 * q4 + e) * STATE;
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], o);
-                float* st = merge + (size_t) (warp * CT + 8 * nt + 2 * q4 + e) * STATE;
-#pragma unroll
-                for (int i = 0; i < STEPS; ++i) *(float2*) (st + 16 * i + 2 * r0) = make_float2(ot[nt][i][e], ot[nt][i][2 + e]);
-                if (r0 == 0) { st[HD] = m[nt][e]; st[HD + 1] = l[nt][e]; st[HD + 2] = mo[nt][e]; }
-            }
+            for (int i = 0; i < STEPS; ++i) *(float2*) (st + 16 * i + 2 * r0) = make_float2(ot[i][e], ot[i][2 + e]);
+            if (r0 == 0) { st[HD] = m[e]; st[HD + 1] = l[e]; st[HD + 2] = mo[e]; }
+        }
         __shared__ float cw_s[FEW_WARPS * CT];
         few_sync();
         if (tid < CT) few_weights<HD, CT>(merge, tid, cw_s, state_s);
@@ -388,21 +375,17 @@ int pattn_few_status() {
     return v;
 }
 
-template <int HD, int NT>
+template <int HD>
 static void launch_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
-    cudaFuncSetAttribute(pattn_few_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<HD, NT>::SMEM);
-    launch(pattn_few_kernel<HD, NT>, (unsigned) pattn_blocks(), FEW_THREADS, Few<HD, NT>::SMEM, s, a, tk, tv);
-    launch_pattn_merge(s, a, pattn_blocks(), Few<HD, NT>::CT);
+    cudaFuncSetAttribute(pattn_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<HD>::SMEM);
+    launch(pattn_few_kernel<HD>, (unsigned) pattn_blocks(), FEW_THREADS, Few<HD>::SMEM, s, a, tk, tv);
+    launch_pattn_merge(s, a, pattn_blocks());
     count_launch(2);
 }
 
-// Sequences of at most PATTN_FEW columns.
 void launch_pattn_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
-    const int group = a.n_head / a.p.n_kv;
-    const bool narrow = (long long) group * a.max_rows <= 8;
-    if (a.p.hd == 128) { if (narrow) launch_few<128, 1>(s, a, tk, tv); else launch_few<128, 2>(s, a, tk, tv); }
-    else if (narrow) launch_few<64, 1>(s, a, tk, tv);
-    else launch_few<64, 2>(s, a, tk, tv);
+    if (a.p.hd == 128) launch_few<128>(s, a, tk, tv);
+    else launch_few<64>(s, a, tk, tv);
 }
 
 }   // namespace nsl

@@ -719,7 +719,7 @@ static void launch_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& t
     const unsigned blocks = (unsigned) sm_count();
     cudaFuncSetAttribute(pattn_many_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<HD>::SMEM);
     launch(pattn_many_kernel<HD, WIDE>, blocks, MANY_THREADS, Many<HD>::SMEM, s, a, tk, tv);
-    const int cols = (a.n_head / a.p.n_kv) * (a.max_rows < a.T ? a.max_rows : a.T);
+    const int cols = (a.n_head / a.p.n_kv) * a.max_rows;
     launch(pattn_join_kernel<HD>, dim3(blocks, (unsigned) (cols < MANY_COLS ? (cols + JOIN_COLS - 1) / JOIN_COLS : MANY_COLS / JOIN_COLS)), JOIN_THREADS, 0, s, a);
     count_launch(2);
 }

@@ -758,3 +758,81 @@ def test_wrapper_refusals():
         with pytest.raises(ValueError):
             call()
     torch.cuda.synchronize()
+
+
+def decode_run(pool, steps, wait, seed):
+    """Store and attend `steps` tokens of three sequences, each step's queries made from the last one's results."""
+    g = gen_of(seed)
+    r = P().Rope(inv_of(64))
+    q = torch.randn(3, 8, 64, generator=g, device="cuda").to(torch.bfloat16)
+    kv = torch.randn(steps, 2, 3, 2, 64, generator=g, device="cuda").to(torch.bfloat16)
+    rows = [ints([[0, 1, 40 + i, 0], [1, 1, 7 + i, 1], [2, 1, 100 + i, 2]]) for i in range(steps)]
+    grow = [ints([[0, 41 + i], [1, 8 + i], [2, 101 + i]]) for i in range(steps)]
+    outs = [torch.empty_like(q) for _ in range(steps)]
+    turned_q = torch.empty_like(q)
+    for i in range(steps):
+        pool.extend(grow[i])
+        pool.append(0, r, q if i == 0 else outs[i - 1], kv[i, 0], kv[i, 1], rows[i], turned_q)
+        pool.attn(0, turned_q, rows[i], outs[i], max_rows=1)
+        if wait:
+            torch.cuda.synchronize()
+    torch.cuda.synchronize()
+    return torch.stack(outs)
+
+
+def test_steps_queued_one_behind_the_other():
+    """Calls that start before their predecessors have ended, whose inputs these write (codes that are then fetched by bulk copies, queries, tables),
+    give what the same calls give one by one, as dependent launches and as ordinary ones."""
+    lib = P().L.load()
+    got = []
+    for wait, mode in ((True, -1), (False, -1), (False, 0), (False, 1)):
+        pool = P().PagePool.empty(1, 60, 2, 64, 16, 3, 12)
+        for t in (pool.k, pool.v):
+            t.zero_()
+        for t in (pool.ks, pool.vs):
+            t.fill_(2.0 ** -6)
+        pool.extend(ints([[0, 40], [1, 7], [2, 100]]))
+        lib.nsl_dependent_launch(mode)
+        try:
+            got.append(decode_run(pool, 40, wait, 31))
+        finally:
+            lib.nsl_dependent_launch(-1)
+    assert all(torch.equal(got[0], x) for x in got[1:])
+    assert bool(torch.isfinite(got[0]).all()) and lib.nsl_pages_attn_status() == 0
+
+
+def test_two_calls_beside_one_another():
+    """Two streams, each with work memory of its own: both give what a call alone gives; few rows and many."""
+    g = gen_of(41)
+    pool = random_pool(g, 2, 700, 2, 128, 16, [3000, 2000, 700])
+    calls = []
+    for seqs in ([[0, 1, 2999, 0], [1, 1, 1999, 1]], [[0, 150, 550, 2], [150, 3, 1900, 1]]):
+        q = torch.randn(153, 16, 128, generator=g, device="cuda").to(torch.bfloat16)
+        calls.append((q, ints(seqs), max(n for _, n, _, _ in seqs), torch.empty_like(pool.attn_work), torch.cuda.Stream(), [torch.zeros_like(q) for _ in range(8)], torch.zeros_like(q)))
+    for q, rows, most, work, _, _, alone in calls:
+        pool.attn(1, q, rows, alone, max_rows=most)
+    torch.cuda.synchronize()
+    for i in range(8):
+        for q, rows, most, work, stream, outs, _ in calls:
+            with torch.cuda.stream(stream):
+                pool.attn(1, q, rows, outs[i], max_rows=most, work=work)
+    torch.cuda.synchronize()
+    for *_, outs, alone in calls:
+        assert all(torch.equal(o, alone) for o in outs)
+
+
+def test_attn_a_sequence_in_several_descriptors():
+    g = gen_of(43)
+    pool = random_pool(g, 2, 20, 2, 64, 64, [900])
+    q = torch.randn(5, 8, 64, generator=g, device="cuda").to(torch.bfloat16)
+    check_attn(pool, q, [[0, 1, 899, 0], [1, 3, 500, 0], [4, 1, 3, 0]])
+    check_attn(pool, q, [[0, 1, 899, 0], [1, 1, 500, 0], [4, 1, 899, 0]])
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_attn_scales_of_either_sign(scale):
+    g = gen_of(44)
+    pool = random_pool(g, 2, 20, 2, 64, 64, [700])
+    q = torch.randn(70, 8, 64, generator=g, device="cuda").to(torch.bfloat16)
+    check_attn(pool, q, [[0, 1, 699, 0]], scale=scale)
+    check_attn(pool, q, [[0, 70, 600, 0]], scale=scale)
