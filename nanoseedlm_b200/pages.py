@@ -48,12 +48,15 @@ def _rows(t, name, like=None):
     shape = t.shape
     if len(shape) != 3:
         raise ValueError(f"{name}: [T][heads][hd], got {tuple(shape)}")
+    T, heads, hd = shape
     rs, hs, es = t.stride()
-    if es != 1 or (shape[1] > 1 and hs != shape[2]):
+    if es != 1 or (hs != hd and heads > 1):
         raise ValueError(f"{name}: dense heads, got strides {t.stride()}")
-    if like is not None and (t.dtype != like.dtype or shape[0] != like.shape[0] or shape[2] != like.shape[2]):
-        raise ValueError(f"{name}: another type, number of rows or head width than the other rows")
-    return rs if shape[0] > 1 else shape[1] * shape[2]
+    if like is not None and like is not t:
+        other = like.shape
+        if T != other[0] or hd != other[2] or t.dtype != like.dtype:
+            raise ValueError(f"{name}: another type, number of rows or head width than the other rows")
+    return rs if T > 1 else heads * hd
 
 
 def _ints(t, name, width):
@@ -80,8 +83,8 @@ def _done():
         raise ValueError(msg.decode())
 
 
-def _stream(index):
-    return torch.cuda.current_stream(index).cuda_stream
+# The stream's handle without a Stream object around it (a microsecond a call), where torch offers that.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _ptr(t):
@@ -95,14 +98,21 @@ def rope(r, q, k, pos, q_out=None, k_out=None, rounded=False):
     index = q.get_device()
     _here(index, k, pos, q_out, k_out, r.inv)
     qs, (T, heads, hd) = _rows(q, "q"), q.shape
-    qos = qs if q_out is q else _rows(q_out, "q_out", q)
-    if q_out.shape != q.shape or _ints(pos, "pos", 0) != T:
-        raise ValueError("q_out: the shape of q; pos: one position a row")
+    qos = qs
+    if q_out is not q:
+        qos = _rows(q_out, "q_out", q)
+        if q_out.shape[1] != heads:
+            raise ValueError("q_out: the shape of q")
+    if _ints(pos, "pos", 0) != T:
+        raise ValueError("pos: one position a row")
     ks = kos = kv = 0
     if k is not None:
-        ks, kos, kv = _rows(k, "k", q), _rows(k_out, "k_out", q), k.shape[1]
-        if k_out.shape != k.shape:
-            raise ValueError("k_out: the shape of k")
+        ks = kos = _rows(k, "k", q)
+        kv = k.shape[1]
+        if k_out is not k:
+            kos = _rows(k_out, "k_out", q)
+            if k_out.shape[1] != kv:
+                raise ValueError("k_out: the shape of k")
     L.load().nsl_rope(_stream(index), r.struct, _type(q, rounded), hd, _ptr(q), qs, _ptr(q_out), qos, heads, _ptr(k), ks, _ptr(k_out), kos, kv, _ptr(pos), T)
     _done()
 
@@ -128,7 +138,6 @@ class PagePool:
         self.work = torch.empty(4 + 3 * shape[1], dtype=torch.int32, device=device)
         self.attn_work = torch.empty(self.lib.nsl_pages_attn_work() // 4, dtype=torch.int32, device=device)
         self.kv, self.hd, self.page = shape[2], shape[4], shape[3]
-        self._heads = (self.kv, self.hd)
         self.struct = L.NslPages(*(t.data_ptr() for t in (k, v, ks, vs, ref, table, length, self.work)), shape[0], shape[1], shape[2], shape[4], shape[3], table.shape[0],
                                table.shape[1], 0)
         self._p = C.byref(self.struct)
@@ -146,14 +155,18 @@ class PagePool:
         descriptors' positions."""
         _here(self.index, q, k, v, rows, q_out, r.inv if r is not None else None)
         q_out = q if q_out is None else q_out
-        ks, vs, T = _rows(k, "k"), _rows(v, "v", k), k.shape[0]
-        if k.shape[1:] != self._heads or v.shape != k.shape:
+        ks, vs, shape = _rows(k, "k"), _rows(v, "v", k), k.shape
+        T = shape[0]
+        if shape[1] != self.kv or shape[2] != self.hd or v.shape[1] != self.kv:
             raise ValueError(f"k, v: [T][{self.kv}][{self.hd}]")
         qs = qos = heads = 0
         if q is not None:
-            qs, qos, heads = _rows(q, "q", k), _rows(q_out, "q_out", k), q.shape[1]
-            if q_out.shape != q.shape:
-                raise ValueError("q_out: the shape of q")
+            qs = qos = _rows(q, "q", k)
+            heads = q.shape[1]
+            if q_out is not q:
+                qos = _rows(q_out, "q_out", k)
+                if q_out.shape[1] != heads:
+                    raise ValueError("q_out: the shape of q")
         n = _ints(rows, "rows", 4)
         self.lib.nsl_pages_append(_stream(self.index), self._p, layer, r.struct if r is not None else _NO_ROPE, _type(k, rounded), _ptr(q), qs, _ptr(q_out), qos, heads, _ptr(k), ks, _ptr(v), vs,
                                   _ptr(rows), n, T)
@@ -163,10 +176,11 @@ class PagePool:
         """The values at the descriptors' positions -> k_out, v_out [T][kv heads][hd]."""
         _here(self.index, rows, k_out, v_out)
         ks, vs = _rows(k_out, "k_out"), _rows(v_out, "v_out", k_out)
-        if k_out.shape[1:] != self._heads or v_out.shape != k_out.shape:
+        shape = k_out.shape
+        if shape[1] != self.kv or shape[2] != self.hd or v_out.shape[1] != self.kv:
             raise ValueError(f"k_out, v_out: [T][{self.kv}][{self.hd}]")
         n = _ints(rows, "rows", 4)
-        self.lib.nsl_pages_read(_stream(self.index), self._p, layer, _type(k_out, rounded), _ptr(k_out), ks, _ptr(v_out), vs, _ptr(rows), n, k_out.shape[0])
+        self.lib.nsl_pages_read(_stream(self.index), self._p, layer, _type(k_out, rounded), _ptr(k_out), ks, _ptr(v_out), vs, _ptr(rows), n, shape[0])
         _done()
 
     def attn(self, layer, q, rows, out, max_rows, scale=None, window=0, work=None):
@@ -174,13 +188,13 @@ class PagePool:
         work memory than the pool's own (int32), for calls that may run beside one another."""
         work = self.attn_work if work is None else work
         _here(self.index, q, rows, out, work)
-        qs, os = _rows(q, "q"), _rows(out, "out")
-        if out.shape != q.shape or q.shape[2] != self.hd:
+        qs, os, (T, heads, hd) = _rows(q, "q"), _rows(out, "out"), q.shape
+        if out.shape != q.shape or hd != self.hd:
             raise ValueError(f"q, out: [T][heads][{self.hd}]")
-        if _ints(work, "work", 0) < self.attn_work.numel():
+        if work is not self.attn_work and _ints(work, "work", 0) < self.attn_work.numel():
             raise ValueError(f"work: {self.attn_work.numel()} ints")
         n = _ints(rows, "rows", 4)
-        self.lib.nsl_pages_attn(_stream(self.index), self._p, layer, _type(q), _ptr(q), qs, q.shape[1], self.hd ** -0.5 if scale is None else scale, window, _ptr(rows), n, max_rows, q.shape[0],
+        self.lib.nsl_pages_attn(_stream(self.index), self._p, layer, _type(q), _ptr(q), qs, heads, hd ** -0.5 if scale is None else scale, window, _ptr(rows), n, max_rows, T,
                                 _type(out, True), _ptr(out), os, _ptr(work))
         _done()
 
