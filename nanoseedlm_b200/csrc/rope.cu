@@ -8,7 +8,7 @@ namespace nsl {
 constexpr int ROPE_THREADS = 128, ROPE_MAX_PAIRS = 256;
 
 // A block takes a row: its (cos, sin) go to shared memory once and serve all heads of q and k; then a thread takes groups of 16
-// values (32 or 64 bytes).  Bound: HBM (5003 rows of 40 heads of 128 bf16 values: 19.4 us = 5.3 TB/s); a decode batch's call is a launch
+// values (32 or 64 bytes).  Bound: HBM (5003 rows of 40 heads of 128 bf16 values: 20.6 us = 5.0 TB/s; two groups a thread in flight: 24.4, fewer blocks an SM); a decode batch's call is a launch
 // (2.3 us).
 template <int TYPE>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(NslRope r, int hd, const void* q, int q_stride, void* qo, int qo_stride, int n_head, const void* k,
