@@ -86,7 +86,7 @@ void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void
  * sequence may appear in several descriptors.
  * Queries take part with 11 significant bits (bf16 values exactly), weights with 11, sums in f32.
  * max_rows: no descriptor has more rows (rows beyond it are left as they are).  work: nsl_pages_attn_work() bytes of device
- * memory, 16-byte aligned, no initial contents; calls that share it run one behind the other, captured ones too.
+ * memory (40 MB for 148 multiprocessors), 16-byte aligned, no initial contents; calls that share it run one behind the other, captured ones too.
  * The step's keys are dealt evenly to the blocks, so a row alone and in a batch may differ in the order of its f32 sums; a call
  * repeated gives the same bits.  n_seqs <= 4096; the 64-key units of a call (all sequences and KV heads) number fewer than 2^31. */
 size_t nsl_pages_attn_work(void);
