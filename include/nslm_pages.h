@@ -62,7 +62,7 @@ typedef struct {
 
 /* One sequence's rows of a call: rows row .. row + rows - 1 of its arrays are positions pos .. pos + rows - 1 of sequence seq.
  * Descriptors come in any order; rows <= 0 is an empty place of a padded batch; a sequence appears once, row ranges do not
- * overlap.  Rows that no descriptor names, or that lie outside [0, T), are left as they are. */
+ * overlap.  Any int32 row and position may be named.  Rows that no descriptor names, or that lie outside [0, T), are left as they are. */
 typedef struct { int32_t row, rows, pos, seq; } NslSeqRows;
 
 /* Queries rotated (q -> qo, see nsl_rope; n_head = 0: none), keys rotated, and keys and values stored in the pages of layer
@@ -71,7 +71,7 @@ typedef struct { int32_t row, rows, pos, seq; } NslSeqRows;
  * call that writes the page's first position and never shrinks until then; when a later row needs a larger one, the codes that
  * are there are rounded to it.  code = x / scale rounded to nearest even; NaN is stored as 0, an infinity as the largest code
  * (its page's scale is then 2^122: the other values of that page and head are lost).  Positions without a page (table entry outside [0, n_pages), position outside the
- * table's row) are not stored.  Pages that several sequences share are not protected here. */
+ * table's row) are not stored; queries at positions below 0 or past 2^31 - 1 are left as they are.  Pages that several sequences share are not protected here. */
 void nsl_pages_append(cudaStream_t s, const NslPages* p, int layer, NslRope r, int type, const void* q, int q_stride, void* qo, int qo_stride, int n_head,
                       const void* k, int k_stride, const void* v, int v_stride, const NslSeqRows* seqs, int n_seqs, int T);
 /* The values at the descriptors' positions -> ko, vo [T][n_kv][hd] (type NSL_F32: code * scale; the others: rounded to bf16).

@@ -14,23 +14,21 @@ namespace nsl {
 
 constexpr int APPEND_THREADS = 256, APPEND_Q_ROWS = 8;      // APPEND_Q_ROWS: of a block at most
 
-// Pages that a descriptor's rows touch; rows outside [0, T) do not count.
+// What of a descriptor is stored: its rows within [0, T) whose positions lie within the table's row.  A descriptor may name any int32 row and
+// position, so the sums are made in 64 bits; what is left fits 32.
 struct SeqSpan { int row, rows, pos; };
-__device__ __forceinline__ SeqSpan span_of(const NslSeqRows& d, int T) {
+__device__ __forceinline__ SeqSpan span_of(const NslSeqRows& d, const NslPages& p, int T) {
+    const long long first = (long long) d.pos - d.row;      // the position that row 0 would have
+    const long long lo = max(max((long long) d.row, 0ll), -first), hi = min(min((long long) d.row + max(d.rows, 0), (long long) T), (long long) p.max_pages * p.page - first);
     SeqSpan s;
-    const int lo = max(d.row, 0), hi = (int) min((long long) d.row + max(d.rows, 0), (long long) T);
-    s.row = lo;
-    s.rows = max(hi - lo, 0);
-    s.pos = d.pos + (lo - d.row);
-    if (s.pos < 0) {      // positions before 0 are nowhere
-        const int cut = (int) min((long long) s.rows, -(long long) s.pos);
-        s.row += cut; s.rows -= cut; s.pos += cut;
-    }
+    s.rows = (int) max(hi - lo, 0ll);
+    s.row = s.rows ? (int) lo : 0;
+    s.pos = s.rows ? (int) (lo + first) : 0;
     return s;
 }
 
 // Unit u of the call: the descriptor and its page, found by a running sum over the descriptors.  -> false: there is none.
-__device__ bool find_unit(const NslSeqRows* seqs, int n_seqs, int T, int page, int u, int* desc, int* nth) {
+__device__ bool find_unit(const NslSeqRows* seqs, int n_seqs, int T, const NslPages& p, int u, int* desc, int* nth) {
     __shared__ int wsum[APPEND_THREADS / 32], at[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) at[0] = -1;
@@ -38,8 +36,8 @@ __device__ bool find_unit(const NslSeqRows* seqs, int n_seqs, int T, int page, i
     for (int i0 = 0; i0 < n_seqs; i0 += APPEND_THREADS) {
         int mine = 0;
         if (i0 + tid < n_seqs) {
-            const SeqSpan s = span_of(seqs[i0 + tid], T);
-            if (s.rows > 0) mine = (s.pos + s.rows - 1) / page - s.pos / page + 1;
+            const SeqSpan s = span_of(seqs[i0 + tid], p, T);
+            if (s.rows > 0) mine = (s.pos + s.rows - 1) / p.page - s.pos / p.page + 1;
         }
         int incl = mine;
 #pragma unroll
@@ -115,9 +113,9 @@ __device__ void append_unit(const AppendArgs& a, int b, float2* cs) {
     const NslPages& p = a.p;
     const int hs = b % a.head_split, is_v = b / a.head_split & 1, u = b / a.head_split >> 1;
     int di, nth;
-    if (!find_unit(a.seqs, a.n_seqs, a.T, p.page, u, &di, &nth)) return;
+    if (!find_unit(a.seqs, a.n_seqs, a.T, p, u, &di, &nth)) return;
     const NslSeqRows d = a.seqs[di];
-    const SeqSpan sp = span_of(d, a.T);
+    const SeqSpan sp = span_of(d, p, a.T);
     const int j = sp.pos / p.page + nth;
     const int lo = max(sp.pos, j * p.page), hi = min(sp.pos + sp.rows, (j + 1) * p.page);      // positions
     const int id = page_of(p, d.seq, j);
@@ -222,7 +220,8 @@ __device__ void append_queries(const AppendArgs& a, int b, float2* cs) {
     row_descriptors(a.seqs, a.n_seqs, t0, n, found);
     if ((int) threadIdx.x < n) {
         const int di = found[threadIdx.x];
-        at[threadIdx.x] = di < 0 ? -1 : a.seqs[di].pos + (t0 + (int) threadIdx.x - a.seqs[di].row);
+        const long long pos = di < 0 ? -1 : (long long) a.seqs[di].pos + (t0 + (int) threadIdx.x) - a.seqs[di].row;
+        at[threadIdx.x] = pos > 0x7FFFFFFF ? -1 : (int) max(pos, -1ll);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < n * pairs; i += APPEND_THREADS) cs[i] = rope_angle(max(at[i / pairs], 0), a.r.inv[i % pairs], a.r.factor);

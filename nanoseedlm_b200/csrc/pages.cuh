@@ -104,7 +104,8 @@ __device__ __forceinline__ void row_descriptors(const NslSeqRows* seqs, int n_se
     __syncthreads();
     for (int i = threadIdx.x; i < n_seqs; i += blockDim.x) {
         const NslSeqRows d = seqs[i];
-        for (int r = max(d.row - t0, 0); r < n && t0 + r - d.row < d.rows; ++r) found[r] = i;
+        const int from = (int) min(max((long long) d.row - t0, 0ll), (long long) n), to = (int) max(min((long long) d.row + max(d.rows, 0) - t0, (long long) n), 0ll);
+        for (int r = from; r < to; ++r) found[r] = i;
     }
     __syncthreads();
 }
