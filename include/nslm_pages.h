@@ -83,7 +83,7 @@ void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void
  * (window <= 0: from 0) of its sequence, query head h over KV head h / (n_head / n_kv).  o = softmax(scale q.k) v, rounded to
  * bf16 (o_type NSL_BF16 or NSL_F32_BF16; o does not overlap q).  Positions without a page are left out, and so is what lies in a
  * page behind the row's position, whatever it holds; a row that nothing is left for gives zeros.  Scales are not negative.  Here a
- * sequence may appear in several descriptors.
+ * sequence may appear in several descriptors, and positions past 2^31 - 1 count as 2^31 - 1.
  * Queries take part with 11 significant bits (bf16 values exactly), weights with 11, sums in f32.
  * max_rows: no descriptor has more rows (rows beyond it are left as they are).  work: nsl_pages_attn_work() bytes of device
  * memory (40 MB for 148 multiprocessors), 16-byte aligned, no initial contents; calls that share it run one behind the other, captured ones too.

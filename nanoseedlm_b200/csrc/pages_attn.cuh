@@ -118,6 +118,13 @@ __device__ __forceinline__ void pattn_warm(const PagesAttn& a) {
         if (at < lines[i]) asm volatile("prefetch.global.L2 [%0];" ::"l"(from[i] + 128 * at));
 }
 
+// The position i rows on; those past 2^31 - 1 count as 2^31 - 1, behind all that a table's row holds.
+__device__ __forceinline__ int pos_of(int pos, int i) { return (int) min((long long) pos + i, 0x7FFFFFFFll); }
+// The first position that the row at position `pos` attends (0 without a window), and one behind its last: both within the table's row.
+__device__ __forceinline__ int first_key(const PagesAttn& a, int pos) {
+    return a.window > 0 ? (int) min(max((long long) pos - a.window + 1, 0ll), (long long) a.p.max_pages * a.p.page) : 0;
+}
+__device__ __forceinline__ int end_key(const PagesAttn& a, int pos) { return max(min(pos, a.p.max_pages * a.p.page - 1) + 1, 0); }
 // A descriptor's rows that exist: [row, row + rows) of the call's rows, the first at position pos.
 struct RowSpan { int row, rows, pos, seq; };
 __device__ __forceinline__ RowSpan row_span(const PagesAttn& a, int i) {
@@ -127,7 +134,7 @@ __device__ __forceinline__ RowSpan row_span(const PagesAttn& a, int i) {
     const long long hi = min((long long) d.row + min(max(d.rows, 0), a.max_rows), (long long) a.T);
     s.row = lo;
     s.rows = (int) max(hi - lo, 0ll);
-    s.pos = d.pos + (lo - d.row);
+    s.pos = (int) min((long long) d.pos + lo - d.row, 0x7FFFFFFFll);
     s.seq = d.seq;
     return s;
 }

@@ -45,9 +45,8 @@ struct FewItem {      // a (sequence, KV head) and the units of it that a block 
 __device__ __forceinline__ int few_units(const PagesAttn& a, const RowSpan& sp, int group, int* k0, int* k1) {
     *k0 = *k1 = 0;
     if (sp.rows <= 0 || sp.rows * group > PATTN_FEW) return 0;
-    const int last = sp.pos + sp.rows;
-    *k1 = max(min(last, a.p.max_pages * a.p.page), 0);
-    *k0 = a.window > 0 ? min(max(sp.pos - a.window + 1, 0), *k1) : 0;
+    *k1 = end_key(a, pos_of(sp.pos, sp.rows - 1));
+    *k0 = min(first_key(a, sp.pos), *k1);
     return max((*k1 + FEW_KEYS - 1) / FEW_KEYS - *k0 / FEW_KEYS, 1);
 }
 
@@ -259,9 +258,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             f[e] = __shfl_sync(0xFFFFFFFFu, fc, 4 * (2 * q4 + e));
-            const int cc = 2 * q4 + e, pos = it.sp.pos + cc / group;
+            const int cc = 2 * q4 + e, pos = pos_of(it.sp.pos, cc / group);
             hi[e] = cc < cols ? pos : -1;
-            lo[e] = a.window > 0 ? pos - a.window + 1 : 0;
+            lo[e] = first_key(a, pos);
         }
         float m[2], mo[2], l[2], ot[STEPS][4];
         m[0] = m[1] = mo[0] = mo[1] = -INFINITY;

@@ -54,8 +54,8 @@ struct ManyItem {
 // Units of column tile ct.
 __device__ __forceinline__ int many_units(const PagesAttn& a, const RowSpan& sp, int group, int cols, int ct, int* k0, int* k1) {
     const int i0 = ct * MANY_COLS / group, i1 = min(cols - 1, ct * MANY_COLS + MANY_COLS - 1) / group;
-    *k1 = max(min(sp.pos + i1 + 1, a.p.max_pages * a.p.page), 0);
-    *k0 = a.window > 0 ? min(max(sp.pos + i0 - a.window + 1, 0), *k1) : 0;
+    *k1 = end_key(a, pos_of(sp.pos, i1));
+    *k0 = min(first_key(a, pos_of(sp.pos, i0)), *k1);
     return max((*k1 + MANY_KEYS - 1) / MANY_KEYS - *k0 / MANY_KEYS, 1);
 }
 __device__ __forceinline__ int warp_sum(int v) {
@@ -337,8 +337,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
             // up to 128 columns: both tiles have them, and every other unit each
             const int shared = it.cols <= MANY_TILE, n = shared ? (it.x1 - it.x0 + 1 - t) / 2 : it.x1 - it.x0, c0 = shared ? 0 : MANY_TILE * t, col = it.col0 + c0 + c;
             const bool valid = c0 + c < it.cols, warp_valid = c0 + 32 * (warp & 3) < it.cols;
-            const int row = it.sp.row + col / group, head = it.kvh * group + col % group, pos = it.sp.pos + col / group;
-            const int hi = valid ? pos : -1, lo = valid && a.window > 0 ? pos - a.window + 1 : 0;
+            const int row = it.sp.row + col / group, head = it.kvh * group + col % group, pos = pos_of(it.sp.pos, col / group);
+            const int hi = valid ? pos : -1, lo = valid ? first_key(a, pos) : 0;
             float f = 0.0f;      // scale, log2 e and the power of two that the query is divided by
             if (warp_valid) {
                 f = many_query<HD>(a, (size_t) row * a.q_stride + (size_t) head * HD, valid, t == 0 ? lanes + TM_Q : 0u, base + F::OFF_Q + c * 128, c & 7);
