@@ -53,13 +53,13 @@ __device__ __forceinline__ void store8(void* base, size_t at, const float* x) {
 }
 
 // (factor cos a, factor sin a) for a = pos * inv, each rounded to f32 once.  The product of an int32 and an f32 has at most 55
-// significant bits; an f32 product would be off by pos * inv * 2^-24, 0.06 at a million positions.  In f64: reduced by the nearest
-// multiple of pi / 2 (in two parts: exact to 1e-16 for every position), then the Taylor sums of sine and cosine on [-pi/4, pi/4]
-// (first terms left out: r^13 / 13!, r^12 / 12!, below 2e-10), a quarter turn at a time.  Keys that lie at the border between two
+// significant bits; an f32 product would be off by pos * inv * 2^-24, 0.06 at a million positions.  In f64: the product and what its rounding left off
+// (`low`; 0 below position 2^29), reduced by the nearest multiple of pi / 2 (in two parts: to 1e-15 for every position), then the Taylor sums of sine and cosine on
+// [-pi/4, pi/4] (first terms left out: r^13 / 13!, r^12 / 12!, below 1.2e-10), a quarter turn at a time.  Keys that lie at the border between two
 // codes then fall as the formula has them.
 __device__ __forceinline__ float2 rope_angle(int pos, float inv, float factor) {
-    const double a = (double) pos * (double) inv, k = rint(a * 0.63661977236758134);
-    const double r = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, a)), z = r * r;
+    const double a = (double) pos * (double) inv, low = fma((double) pos, (double) inv, -a), k = rint(a * 0.63661977236758134);
+    const double r = fma(-k, 6.123233995736766e-17, fma(-k, 1.5707963267948966, a)) + low, z = r * r;
     const double sn = fma(r * z, fma(z, fma(z, fma(z, fma(z, -1.0 / 39916800.0, 1.0 / 362880.0), -1.0 / 5040.0), 1.0 / 120.0), -1.0 / 6.0), r);
     const double cs = fma(z, fma(z, fma(z, fma(z, fma(z, -1.0 / 3628800.0, 1.0 / 40320.0), -1.0 / 720.0), 1.0 / 24.0), -0.5), 1.0);
     const int q = (int) ((long long) k & 3);

@@ -1,9 +1,12 @@
 """The paged cache at the ends of its ranges, on the GPU.
 
 Roundings that the tolerances count (half a step each, relative): f32 2^-24, bf16 2^-8, f16 2^-11."""
+import math
+from fractions import Fraction
+
 import pytest
 import torch
-from test_gpu_pages import BF16, attn64, gen_of, ints, random_pool
+from test_gpu_pages import BF16, F32, P, attn64, gen_of, ints, inv_of, random_pool, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +64,42 @@ def test_attn_at_positions_that_wrap(rows, page):
         w, s = attn64(pool, 1, q, [[i, 1, 100000, 0]], 0.125, 100001 - lo)
         want, size = want + w, size + s
     assert bool(((o.double() - want).abs() <= BF16 * want.abs() + (1 + BF16) * WEIGHTS * size)[:rows].all())
+
+
+# ---- angles of far positions ------------------------------------------------------------------------------------------------------
+PI = Fraction(314159265358979323846264338327950288419716939937510582097494459230781640628620899, 10 ** 80)
+
+
+@pytest.mark.parametrize("first", [-2 ** 31, 2 ** 29 + 1, 2 ** 30 + 3, LAST - 63])
+def test_rope_angles_are_exact(first):
+    """cos and sin of pos * inv, the product and its reduction to a quarter turn in exact fractions.  The result is rounded to f32 once (2^-24 of it); sums of Taylor
+    terms up to r^11 and r^10 leave out at most (pi/4)^12 / 12! < 1.2e-10, and a few roundings in 64 bits, 1e-15."""
+    vals = [1.0, 0.7310585786300049, 0.99999994, 1e-3, 0.5000001, 0.1234567, 3e-5, 0.9] + [10000.0 ** (-2 * p / 16) * 0.9876543 for p in range(8)]
+    inv = torch.tensor(vals, dtype=torch.float32)
+    pos = list(range(first, first + 64))
+    x = torch.zeros(64, 1, 64, device="cuda")
+    x[..., :16] = 1.0      # pairs (1, 0): the rotated pair is (cos, sin)
+    P().rope(P().Rope(inv.cuda()), x, None, ints(pos))
+    got = x.cpu().double()
+    for t, p in enumerate(pos):
+        for i in range(16):
+            a = Fraction(p) * Fraction(float(inv[i]))
+            k = round(a / (PI / 2))
+            r = float(a - k * PI / 2)
+            c, s = [(math.cos(r), math.sin(r)), (-math.sin(r), math.cos(r)), (-math.cos(r), -math.sin(r)), (math.sin(r), -math.cos(r))][k % 4]
+            assert abs(float(got[t, 0, i]) - c) <= F32 * abs(c) + 1.3e-10, (p, i)
+            assert abs(float(got[t, 0, i + 16]) - s) <= F32 * abs(s) + 1.3e-10, (p, i)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("hd,rot,factor", [(64, 64, 1.0), (128, 64, 1.25), (256, 256, 1.0)])
+def test_rope_rounds_each_step_once(hd, rot, factor, inter):
+    """Sine and cosine times the factor, the two products and their sum: 3 roundings to f32 of factor (|u| + |w|) at most, and 1.2e-10 of it from the Taylor sums."""
+    g = gen_of(55)
+    x = torch.randn(500, 3, hd, generator=g, device="cuda")
+    pos = torch.randint(0, 2 ** 29, (500,), generator=g, device="cuda", dtype=torch.int32)
+    r = P().Rope(inv_of(rot), interleaved=inter, factor=factor)
+    out = torch.empty_like(x)
+    P().rope(r, x, None, pos, out)
+    want, size = turned(x, pos, r.inv, inter, factor)
+    assert bool(((out.double() - want).abs() <= 3.01 * F32 * factor * size).all())
