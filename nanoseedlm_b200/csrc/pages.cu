@@ -358,9 +358,9 @@ __global__ void __launch_bounds__(MAN_THREADS) extend_kernel(NslPages p, const N
     if (fits) {
         old = p.len[seq];
         now = max(now, old);
-        have = pages_for(old, p.page);
+        have = pages_for(max(old, 0), p.page);
         need = pages_for(now, p.page);
-        fits = need <= p.max_pages && old >= 0;
+        fits = need <= p.max_pages && old >= 0;      // (a length below 0 is no length: refused, and no entry before the row is reached)
     }
     if (fits && now > old && old % p.page) {
         last_id = page_of(p, seq, old / p.page);

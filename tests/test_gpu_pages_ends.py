@@ -103,3 +103,24 @@ def test_rope_rounds_each_step_once(hd, rot, factor, inter):
     P().rope(r, x, None, pos, out)
     want, size = turned(x, pos, r.inv, inter, factor)
     assert bool(((out.double() - want).abs() <= 3.01 * F32 * factor * size).all())
+
+
+# ---- lengths that are none ----------------------------------------------------------------------------------------------------------
+def test_management_of_a_length_below_zero():
+    """A sequence whose length the host has spoilt: its requests are refused, nobody else's page or entry changes."""
+    pool = P().PagePool.empty(1, 40, 1, 64, 16, 3, 10)
+    got = ints([7, 7, 7])
+    pool.extend(ints([[0, 160], [1, 20], [2, 20]]), got)
+    pool.length[1] = -100
+    table, ref = pool.table.clone(), pool.ref.clone()
+    pool.extend(ints([[1, 50], [2, 40], [0, 161]]), got)
+    assert got.tolist() == [0, 1, 0]
+    pool.trim(ints([[1, 0]]))
+    pool.fork(ints([[1, 2, 5, 0]]))
+    assert pool.length.tolist() == [160, -100, 40]
+    table[2, 2] = pool.table[2, 2]
+    ref[pool.table[2, 2]] = 1
+    assert torch.equal(pool.table, table) and torch.equal(pool.ref, ref)
+    pool.length[1] = 2 ** 31 - 1
+    pool.extend(ints([[1, 50], [2, 5], [0, 3]]), got)
+    assert got.tolist() == [0, 1, 1] and torch.equal(pool.table, table) and torch.equal(pool.ref, ref)
