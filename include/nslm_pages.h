@@ -92,11 +92,16 @@ void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void
 size_t nsl_pages_attn_work(void);
 void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, const void* q, int q_stride, int n_head, float scale, int window,
                     const NslSeqRows* seqs, int n_seqs, int max_rows, int T, int o_type, void* o, int o_stride, void* work);
-/* 0, or the code of the first bounded device-side wait that ran out in an attention block since the last call (few rows: 1 a fetch
- * waiting for a free stage, 2 a computing warp waiting for a full one; many rows: 4 .. 6 the softmax waiting for scores, for
- * scales or for values added, 7 and 8 the expansion for codes or a free tile, 9 a fetch, 10 .. 13 the issue of products for
- * queries, tiles, read scores or weights); the results of such a block are not valid.  Call after synchronising. */
+/* 0, or the code of the first bounded device-side wait that ran out (after a second) in an attention block since it was last reported (few
+ * rows: 1 a fetch waiting for a free stage, 2 a computing warp waiting for a full one; many rows: 4 .. 6 the softmax waiting
+ * for scores, for scales or for values added, 7 and 8 the expansion for codes or a free tile, 9 a fetch, 10 .. 13 the issue of
+ * products for queries, tiles, read scores or weights).  What such a block had not finished by then is NaN in the results.  A call reports one
+ * code: where both kinds of block had one, the next call reports the other.  -1, with a message: the device cannot be read.
+ * Synchronous; call it after the stream has drained. */
 int nsl_pages_attn_status(void);
+/* For testing what a host does about that: until it is called with 0, this thread's nsl_pages_attn calls fetch no codes, so
+ * every wait for some runs out, after wait_ns (a second at most), and their results are NaN. */
+void nsl_pages_attn_hold(unsigned long long wait_ns);
 
 /* ---- management: device lists, at most NSL_PAGES_LIST entries a call; the calls on a pool run one behind the other -------- */
 #define NSL_PAGES_LIST 1024

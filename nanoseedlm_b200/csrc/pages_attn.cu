@@ -126,9 +126,12 @@ extern "C" {
 size_t nsl_pages_attn_work(void) { return (size_t) pattn_blocks() * 16 + (size_t) sm_count() * 2 * PATTN_MANY * PATTN_STATE<128> * 4; }
 
 int nsl_pages_attn_status(void) {
-    const int few = pattn_few_status(), many = pattn_many_status();
-    return few ? few : many;
+    const int few = pattn_few_status();
+    return few ? few : pattn_many_status();
 }
+
+static thread_local unsigned long long tl_hold_ns = 0;
+void nsl_pages_attn_hold(unsigned long long wait_ns) { tl_hold_ns = wait_ns < PATTN_WAIT_NS ? wait_ns : PATTN_WAIT_NS; }
 
 void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, const void* q, int q_stride, int n_head, float scale, int window,
                     const NslSeqRows* seqs, int n_seqs, int max_rows, int T, int o_type, void* o, int o_stride, void* work) {
@@ -149,6 +152,8 @@ void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, co
     a.part = (float*) ((char*) work + 16 * (size_t) pattn_blocks());
     a.scale = scale; a.q_type = q_type; a.q_stride = q_stride; a.o_type = o_type; a.o_stride = o_stride;
     a.n_head = n_head; a.layer = layer; a.window = window; a.n_seqs = n_seqs; a.max_rows = max_rows < T ? max_rows : T; a.T = T;
+    a.hold = tl_hold_ns > 0;
+    a.wait_ns = a.hold ? tl_hold_ns : PATTN_WAIT_NS;
     // One of the two for all sequences of a call.  The few-row kernel reads the keys for 8 columns at a time, the wide one makes a tile of 128
     // whatever it holds: 32 rows of 4096 keys with 8 heads a KV head 21 against 49 us, with 16 columns (two passes' registers) 57 against
     // 51, 8 rows with 16 heads 32 against 29.  Beside a prompt's rows decode rows cost less in the wide kernel's blocks than two more launches.

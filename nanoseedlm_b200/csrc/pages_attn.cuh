@@ -17,6 +17,8 @@ struct PagesAttn {
     int4* rec;          // per block, its item that ends in a later block: states | KV head << 16 (0: none), first row, first column, columns
     float scale;
     int q_type, q_stride, o_type, o_stride, n_head, layer, window, n_seqs, max_rows, T;
+    int hold;                      // no block fetches anything (nsl_pages_attn_hold)
+    unsigned long long wait_ns;    // how long a wait lasts at most
 };
 
 // Blocks of a launch at most: two an SM (their number fits a record's 16 bits).
@@ -25,7 +27,8 @@ constexpr int PATTN_FEW = 8, PATTN_MANY = 256;      // columns of an item
 template <int HD>
 constexpr int PATTN_STATE = HD + 4;      // floats of a column's state: O [HD], m, l, mo, one unused
 void launch_pattn_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv);
-int pattn_few_status();
+constexpr unsigned long long PATTN_WAIT_NS = 1000000000ull;
+int pattn_few_status();      // 0, a wait's code, or -1; a code is read once
 int pattn_many_status();
 void launch_pattn_merge(cudaStream_t s, const PagesAttn& a, int blocks);
 
@@ -34,7 +37,6 @@ void launch_pattn_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk,
 
 #ifdef __CUDACC__
 constexpr uint32_t PATTN_WAIT_LIMIT = 1u << 24;
-constexpr unsigned long long PATTN_WAIT_NS = 1000000000ull;
 
 __device__ __forceinline__ uint32_t pa_smem(const void* p) { return (uint32_t) __cvta_generic_to_shared(p); }
 __device__ __forceinline__ void pa_bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
@@ -50,11 +52,12 @@ __device__ __forceinline__ bool pa_bar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// Waits are bounded: after PATTN_WAIT_NS or PATTN_WAIT_LIMIT attempts a wait sets the block's abort flag and a status code and returns,
-// and so does every later wait of the block at once.  The block then runs to its end on what is there (every access in bounds,
-// every barrier met), fetches nothing more, and its results are not valid.  A wait that returned whether it succeeded, voted on by
-// the warp, cost a unit of 256 columns a third of its time.
-static __device__ __noinline__ void pa_bar_wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+// Waits are bounded: after wait_ns (PATTN_WAIT_NS) or PATTN_WAIT_LIMIT attempts a wait sets the block's abort flag and a status code and
+// returns, and so does every later wait of the block at once.  The block then runs to its end on what is there (every access in
+// bounds, every barrier met), fetches nothing more, and gives a sum l of NaN with every item that it has not finished by then, so
+// that its results, and those that its states are joined into, are NaN.  A wait that returned whether it succeeded, voted on
+// by the warp, cost a unit of 256 columns a third of its time.
+static __device__ __noinline__ void pa_bar_wait_long(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code, unsigned long long wait_ns) {
     unsigned long long t0 = 0;
     for (uint32_t i = 0; i < PATTN_WAIT_LIMIT; ++i) {
         if (*abort_flag || pa_bar_try(bar, parity)) return;
@@ -62,14 +65,14 @@ static __device__ __noinline__ void pa_bar_wait_long(uint32_t bar, uint32_t pari
             unsigned long long t;
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
             if (!t0) t0 = t;
-            if (t - t0 > PATTN_WAIT_NS) break;
+            if (t - t0 > wait_ns) break;
         }
     }
     *abort_flag = 1;
     atomicCAS(status, 0, code);
 }
-__device__ __forceinline__ void pa_bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-    if (!pa_bar_try(bar, parity) && !pa_bar_try(bar, parity) && !pa_bar_try(bar, parity)) pa_bar_wait_long(bar, parity, abort_flag, status, code);
+__device__ __forceinline__ void pa_bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code, unsigned long long wait_ns) {
+    if (!pa_bar_try(bar, parity) && !pa_bar_try(bar, parity) && !pa_bar_try(bar, parity)) pa_bar_wait_long(bar, parity, abort_flag, status, code, wait_ns);
     __syncwarp();
 }
 __device__ __forceinline__ void pa_tma_rows(uint32_t smem, const CUtensorMap* tm, int row, uint32_t bar) {      // x = 0: the rows' first code
@@ -138,12 +141,22 @@ __device__ __forceinline__ RowSpan row_span(const PagesAttn& a, int i) {
     s.seq = d.seq;
     return s;
 }
-// What a column's O is multiplied with: 2^(mo - m) / l; nothing attended: 0.
-__device__ __forceinline__ float pattn_factor(float m, float l, float mo) { return l == 0.0f || mo == -INFINITY ? 0.0f : pa_ex2(mo - m) / l; }
+// What a column's O is multiplied with: 2^(mo - m) / l; nothing attended: 0; a sum that is NaN stays NaN.
+__device__ __forceinline__ float pattn_factor(float m, float l, float mo) { return l != l ? l : l == 0.0f || mo == -INFINITY ? 0.0f : pa_ex2(mo - m) / l; }
 __device__ __forceinline__ void store_bf16_of(const PagesAttn& a, size_t at, float x) {
     const uint32_t b = bf16_pair(x, 0.0f);
     if (a.o_type == NSL_BF16) ((uint16_t*) a.o)[at] = (uint16_t) b;
     else ((float*) a.o)[at] = __uint_as_float(b << 16);
+}
+// A status word read and, if it holds a code, cleared; -1: it cannot be read.
+inline int pattn_status_of(int& word) {
+    int v = 0;
+    const int zero = 0;
+    if (cudaMemcpyFromSymbol(&v, word, sizeof v) != cudaSuccess || (v && cudaMemcpyToSymbol(word, &zero, sizeof zero) != cudaSuccess)) {
+        set_error("nsl_pages_attn_status: the status word cannot be read");
+        return -1;
+    }
+    return v;
 }
 #endif
 

@@ -169,13 +169,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
     FewWalk walk = {plan[0], plan[1]};
     FewItem it;
     int stage = 0, round = 0;      // the ring's next stage, and how often it has been round
-    auto wait = [&](uint32_t bar, uint32_t parity, int code) { pa_bar_wait(bar, parity, &abort_flag, &g_pattn_status, code); };
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) { pa_bar_wait(bar, parity, &abort_flag, &g_pattn_status, code, a.wait_ns); };
     const int piece = min(a.p.page, FEW_KEYS), pieces = FEW_KEYS / piece;      // rows of a piece, pieces of a unit
 
     if (warp == FEW_WARPS) {      // ---- fetches ----
         asm volatile("fence.proxy.async;" ::: "memory");      // codes that the kernel before has stored
         const int batch = 32 / pieces;      // units a look ahead covers
-        int x = x0;
+        int x = a.hold ? xe : x0;
         while (walk.next(a, group, x, xe, &it)) {
             const size_t head_at = (size_t) a.layer * a.p.n_pages * a.p.n_kv + it.kvh;
             for (int b = it.x0; b < it.x1; b += batch) {
@@ -348,7 +348,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
         }
         __shared__ float cw_s[FEW_WARPS * CT];
         few_sync();
-        if (tid < CT) few_weights<HD, CT>(merge, tid, cw_s, state_s);
+        if (tid < CT) {
+            few_weights<HD, CT>(merge, tid, cw_s, state_s);
+            if (*(volatile int*) &abort_flag) state_s[3 * tid + 1] = NAN;      // a wait of the block has run out
+        }
         few_sync();
         const int b0 = it.first / per, b1 = (it.first + it.units - 1) / per, parts = b1 - b0 + 1;
         float* const mine = a.part + (size_t) (2 * blockIdx.x + ((int) blockIdx.x == b0)) * CT * STATE;
@@ -368,12 +371,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
     }
 }
 
-int pattn_few_status() {
-    int v = 0, zero = 0;
-    cudaMemcpyFromSymbol(&v, g_pattn_status, sizeof v);
-    if (v) cudaMemcpyToSymbol(g_pattn_status, &zero, sizeof zero);
-    return v;
-}
+int pattn_few_status() { return pattn_status_of(g_pattn_status); }
 
 template <int HD>
 static void launch_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {

@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
     __syncthreads();
     ManyWalk walk = {plan[0], plan[1]};
     ManyItem it;
-    auto wait = [&](uint32_t bar, uint32_t parity, int code) { pa_bar_wait(bar, parity, &abort_flag, &g_pattn_many_status, code); };
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) { pa_bar_wait(bar, parity, &abort_flag, &g_pattn_many_status, code, a.wait_ns); };
     int g = 0;      // units this block has done: the rings' position
 
     if (warp < MANY_EXPAND) {      // ---- softmax: tile t, column c of it ----
@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
                     mo = mmo;
                 }
             }
+            if (*(volatile int*) &abort_flag) l = NAN;      // a wait of the block has run out
             if (warp_valid && !(shared && t)) {
                 const bool second = shared && it.x1 - it.x0 > 1;      // (an O that nothing was added to holds anything)
                 if (parts == 1) { const float fac = pattn_factor(m, l, mo); by *= fac; by1 *= fac; }
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
         asm volatile("fence.proxy.async;" ::: "memory");      // codes that the kernel before has stored
         const int piece = min(a.p.page, MANY_KEYS), pieces = MANY_KEYS / piece, batch = 32 / pieces;
         float4* const meta_to = (float4*) (smem + F::OFF_META);
-        for (int x = x0; walk.next(a, group, x, xe, &it); x = it.x1) {
+        for (int x = a.hold ? xe : x0; walk.next(a, group, x, xe, &it); x = it.x1) {
             const size_t head_at = (size_t) a.layer * a.p.n_pages * a.p.n_kv + it.kvh;
             for (int b = it.x0; b < it.x1; b += batch) {
                 const int p = (it.tile0 + b - it.first) * MANY_KEYS + lane * piece;      // lane j: piece j from here on
@@ -646,12 +647,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
     if (warp == MANY_SCORES) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_slot) : "memory");
 }
 
-int pattn_many_status() {
-    int v = 0, zero = 0;
-    cudaMemcpyFromSymbol(&v, g_pattn_many_status, sizeof v);
-    if (v) cudaMemcpyToSymbol(g_pattn_many_status, &zero, sizeof zero);
-    return v;
-}
+int pattn_many_status() { return pattn_status_of(g_pattn_many_status); }
 
 // The states of an unfinished item joined.  Block (b, y): the item that block b leaves unfinished, columns 32 y .. 32 y + 31; a lane a
 // column, a warp an eighth of the dims, so the states are read as they were written, 128 bytes a warp; the results are turned

@@ -211,6 +211,7 @@ PROTOTYPES = {
     "nsl_pages_attn_work": (_sz, []),
     "nsl_pages_attn": (None, [_vp, _vp, _i, _i, _vp, _i, _i, C.c_float, _i, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
     "nsl_pages_attn_status": (_i, []),
+    "nsl_pages_attn_hold": (None, [C.c_uint64]),
     "nsl_pages_extend": (None, [_vp, _vp, _vp, _i, _vp]),
     "nsl_pages_fork": (None, [_vp, _vp, _vp, _i]),
     "nsl_pages_trim": (None, [_vp, _vp, _vp, _i]),

@@ -185,7 +185,8 @@ class PagePool:
 
     def attn(self, layer, q, rows, out, max_rows, scale=None, window=0, work=None):
         """Causal attention of q [T][heads][hd] over the sequences' pages -> out (bfloat16, or float32 rounded to bf16).  work: other
-        work memory than the pool's own (int32), for calls that may run beside one another."""
+        work memory than the pool's own (int32), for calls that may run beside one another.  NaN in a row whose query is finite: a wait on the
+        device ran out, see status()."""
         work = self.attn_work if work is None else work
         _here(self.index, q, rows, out, work)
         qs, os, (T, heads, hd) = _rows(q, "q"), _rows(out, "out"), q.shape
@@ -197,6 +198,15 @@ class PagePool:
         self.lib.nsl_pages_attn(_stream(self.index), self._p, layer, _type(q), _ptr(q), qs, heads, hd ** -0.5 if scale is None else scale, window, _ptr(rows), n, max_rows, T,
                                 _type(out, True), _ptr(out), os, _ptr(work))
         _done()
+
+    def status(self):
+        """0, or the code of a wait that ran out in an attention call (see nsl_pages_attn_status); reading clears it.  Synchronises the device."""
+        torch.cuda.synchronize(self.device)
+        with torch.cuda.device(self.device):
+            code = self.lib.nsl_pages_attn_status()
+        if code < 0:
+            raise RuntimeError(L.last_error() or "nsl_pages_attn_status failed")
+        return code
 
     def extend(self, reqs, got=None):
         """Sequences grow: reqs int32 [n][2] = (sequence, length); got (int32 [n], optional): 1 where served."""

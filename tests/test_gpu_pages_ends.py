@@ -6,7 +6,7 @@ from fractions import Fraction
 
 import pytest
 import torch
-from test_gpu_pages import BF16, F32, P, attn64, gen_of, ints, inv_of, random_pool, turned
+from test_gpu_pages import BF16, F32, P, attn64, check_attn, gen_of, ints, inv_of, random_pool, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +124,44 @@ def test_management_of_a_length_below_zero():
     pool.length[1] = 2 ** 31 - 1
     pool.extend(ints([[1, 50], [2, 5], [0, 3]]), got)
     assert got.tolist() == [0, 1, 1] and torch.equal(pool.table, table) and torch.equal(pool.ref, ref)
+
+
+# ---- waits that run out -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,group,hd,page,code", [(1, 8, 128, 64, 2), (2, 4, 64, 16, 2), (3, 8, 64, 32, 7), (20, 2, 128, 128, 7), (200, 4, 128, 64, 7)], ids=str)
+def test_attn_wait_that_runs_out(rows, group, hd, page, code):
+    """Codes that are never fetched: every block's wait for them ends after its bound, the results are NaN and the status says why, rows that nobody
+    names stay, and the next call is right."""
+    lib = P().L.load()
+    g = gen_of(56 + rows)
+    lengths = [3000, 400, 70 + rows]
+    pool = random_pool(g, 2, sum(-(-n // page) for n in lengths), 2, hd, page, lengths)
+    q = torch.randn(3 * rows + 2, 2 * group, hd, generator=g, device="cuda").to(torch.bfloat16)
+    seqs = [[i * rows, rows, n - rows, i] for i, n in enumerate(lengths)]
+    check_attn(pool, q, seqs)
+    assert pool.status() == 0
+    o = torch.full_like(q, 5.0)
+    lib.nsl_pages_attn_hold(3_000_000)      # ns
+    try:
+        pool.attn(1, q, ints(seqs), o, max_rows=rows)
+        torch.cuda.synchronize()
+    finally:
+        lib.nsl_pages_attn_hold(0)
+    assert bool(o[:3 * rows].isnan().all()) and bool((o[3 * rows:] == 5.0).all())
+    got = pool.status()
+    assert got == code if code == 2 else 4 <= got <= 13      # many rows: whichever of the block's warps gave up first
+    assert pool.status() == 0
+    check_attn(pool, q, seqs)
+    assert pool.status() == 0
+
+
+def test_attn_status_reports_both_kinds_of_block():
+    lib = P().L.load()
+    pool = random_pool(gen_of(57), 1, 10, 1, 64, 16, [100])
+    q = torch.ones(20, 4, 64, device="cuda")
+    lib.nsl_pages_attn_hold(1_000_000)
+    try:
+        pool.attn(0, q, ints([[0, 1, 99, 0]]), torch.empty_like(q), max_rows=1)
+        pool.attn(0, q, ints([[0, 20, 80, 0]]), torch.empty_like(q), max_rows=20)
+    finally:
+        lib.nsl_pages_attn_hold(0)
+    assert pool.status() == 2 and 4 <= pool.status() <= 13 and pool.status() == 0
