@@ -91,7 +91,10 @@ __device__ __forceinline__ uint32_t few_turn(uint32_t x) {      // an 8 x 8 tile
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-__device__ __forceinline__ void few_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_WARPS) : "memory"); }      // the computing warps
+__device__ __forceinline__ void few_sync() {      // the computing warps; the barrier is each whole warp's, and is reached from branches of single lanes
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_WARPS) : "memory");
+}
 
 // Column c's weights of the warps' states: cw[w * CT + c] = 2^(mo_w - mo); and m, l, mo of all.
 template <int HD, int CT>
@@ -192,7 +195,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
                 const int row = id < 0 ? -1 : (int) ((head_at + (size_t) id * a.p.n_kv) * a.p.page + p % a.p.page);
                 for (int u = 0; u < batch && b + u < it.x1; ++u) {
                     if (round > 0) wait(empty + 8 * stage, (round - 1) & 1, 1);
-                    if (*(volatile int*) &abort_flag) break;
+                    if (__any_sync(0xFFFFFFFFu, *(volatile int*) &abort_flag)) break;      // by all lanes or none
                     const int from = u * pieces + (lane & (pieces - 1)), of_group = u * pieces + (lane & 3) * 16 / piece;
                     const int my_row = __shfl_sync(0xFFFFFFFFu, row, from), g_row = __shfl_sync(0xFFFFFFFFu, row, of_group);
                     const float g_ks = __shfl_sync(0xFFFFFFFFu, ks, of_group), g_lv = __shfl_sync(0xFFFFFFFFu, lv, of_group);
@@ -316,6 +319,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
 #pragma unroll
                     for (int i = 0; i < STEPS; ++i) { ot[i][0] *= cor[0]; ot[i][1] *= cor[1]; ot[i][2] *= cor[0]; ot[i][3] *= cor[1]; }
                 }
+                __syncwarp();      // lanes that had a maximum move and lanes that had none: what follows is the whole warp's
                 pw[0] = few_turn(pa_f16x2(w[0], w[1]));
                 pw[1] = few_turn(pa_f16x2(w[2], w[3]));
 #pragma unroll

@@ -214,6 +214,7 @@ static __device__ __noinline__ float many_query(const PagesAttn& a, size_t at, b
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = pa_f16x2(v[2 * e] * inv, v[2 * e + 1] * inv);
+        __syncwarp();      // lanes with and without a column: the store is the whole warp's
         if (tq) tm_st16(tq + d / 2, w);
         else {
 #pragma unroll
@@ -232,6 +233,7 @@ static __device__ __noinline__ void many_results(const PagesAttn& a, uint32_t to
 #pragma unroll 1
     for (int d = 0; d < HD; d += 16) {
         uint32_t v[16], v1[16];
+        __syncwarp();      // lanes with and without a column: the load is the whole warp's
         tm_ld16(to + d, v);
         if (second) tm_ld16(to + 128 + d, v1);
         if (!valid) continue;
@@ -534,6 +536,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
                 }
             }
             // values, transposed: 16 keys a warp, 32 dims a step -> rows of 64 keys
+            __syncwarp();      // the two ways round of the keys' pieces: the loads are the whole warp's
 #pragma unroll
             for (int j = 0; j < HD / 16; j += 2) {
                 uint32_t c[4];
@@ -567,7 +570,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
                 for (int u = 0; u < batch && b + u < it.x1; ++u, ++g) {
                     const uint32_t rs = (uint32_t) (g % MANY_RAW);
                     if (g >= MANY_RAW) wait(raw_empty + 8 * rs, (g / MANY_RAW - 1) & 1, 9);
-                    if (*(volatile int*) &abort_flag) break;
+                    if (__any_sync(0xFFFFFFFFu, *(volatile int*) &abort_flag)) break;      // by all lanes or none
                     const int from = u * pieces + (lane & (pieces - 1)), of_group = u * pieces + (lane & 3) * 16 / piece;
                     const int my_row = __shfl_sync(0xFFFFFFFFu, row, from), g_row = __shfl_sync(0xFFFFFFFFu, row, of_group);
                     const float g_ks = __shfl_sync(0xFFFFFFFFu, ks, of_group), g_lv = __shfl_sync(0xFFFFFFFFu, lv, of_group);
@@ -643,6 +646,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
     }
     tm_before();
     __syncthreads();
+    __syncwarp();
     tm_after();
     if (warp == MANY_SCORES) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_slot) : "memory");
 }

@@ -6,7 +6,7 @@ from fractions import Fraction
 
 import pytest
 import torch
-from test_gpu_pages import BF16, F32, P, attn64, check_attn, gen_of, ints, inv_of, random_pool, turned
+from test_gpu_pages import BF16, F32, P, attn64, check_attn, gen_of, held, ints, inv_of, random_pool, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -165,3 +165,20 @@ def test_attn_status_reports_both_kinds_of_block():
     finally:
         lib.nsl_pages_attn_hold(0)
     assert pool.status() == 2 and 4 <= pool.status() <= 13 and pool.status() == 0
+
+
+# ---- warps that are partly filled ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd,page", [(128, 64), (128, 16), (64, 32), (64, 128)])
+@pytest.mark.parametrize("cols", [1, 3, 7, 8, 9, 15, 17, 31, 33, 47, 65, 96, 100, 127, 129, 130, 161, 200, 255, 257, 300])
+def test_attn_of_any_number_of_columns(cols, hd, page):
+    """Columns that end anywhere in a warp, some of which have their maxima move with every unit and others only with the first."""
+    g = gen_of(cols + hd)
+    n = max(500, cols + 200)
+    pool = random_pool(g, 2, -(-n // page) + 1, 2, hd, page, [n])
+    q = torch.randn(cols + 1, 2, hd, generator=g, device="cuda")
+    k = held(pool, 1, 0, n)[0].float()      # [n][2][hd]
+    grow = torch.arange(n, device="cuda")[:, None, None] / n
+    pool.k[1, pool.table[0].long()] = 0
+    pool.append(1, None, None, (k * grow ** 2).contiguous(), (torch.randn(n, 2, hd, generator=g, device="cuda")).contiguous(), ints([[0, n, 0, 0]]))
+    q[::3] *= 0.01
+    check_attn(pool, q.to(torch.bfloat16), [[0, cols, n - cols, 0]])
