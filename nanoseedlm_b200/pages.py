@@ -85,6 +85,7 @@ def _done():
 
 # The stream's handle without a Stream object around it (a microsecond a call), where torch offers that.
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 
 
 def _ptr(t):
@@ -141,6 +142,16 @@ class PagePool:
         self.struct = L.NslPages(*(t.data_ptr() for t in (k, v, ks, vs, ref, table, length, self.work)), shape[0], shape[1], shape[2], shape[4], shape[3], table.shape[0],
                                table.shape[1], 0)
         self._p = C.byref(self.struct)
+        self._works = {_stream(self.index): self.attn_work}      # by stream: calls on one run one behind the other
+
+    def _work_of(self, stream):
+        """Attention's work memory: the stream's own, made at its first call; in a capture the graph's, from the capture's memory."""
+        if _capturing():
+            return torch.empty_like(self.attn_work)
+        work = self._works.get(stream)
+        if work is None:
+            work = self._works[stream] = torch.empty_like(self.attn_work)
+        return work
 
     @classmethod
     def empty(cls, layers, pages, kv, hd, page, sequences, max_pages, device="cuda"):
@@ -184,18 +195,20 @@ class PagePool:
         _done()
 
     def attn(self, layer, q, rows, out, max_rows, scale=None, window=0, work=None):
-        """Causal attention of q [T][heads][hd] over the sequences' pages -> out (bfloat16, or float32 rounded to bf16).  work: other
-        work memory than the pool's own (int32), for calls that may run beside one another.  NaN in a row whose query is finite: a wait on the
+        """Causal attention of q [T][heads][hd] over the sequences' pages -> out (bfloat16, or float32 rounded to bf16).  Each stream and each
+        captured graph has work memory of its own (40 MB); work: another one (int32).  NaN in a row whose query is finite: a wait on the
         device ran out, see status()."""
-        work = self.attn_work if work is None else work
         _here(self.index, q, rows, out, work)
         qs, os, (T, heads, hd) = _rows(q, "q"), _rows(out, "out"), q.shape
         if out.shape != q.shape or hd != self.hd:
             raise ValueError(f"q, out: [T][heads][{self.hd}]")
-        if work is not self.attn_work and _ints(work, "work", 0) < self.attn_work.numel():
+        if work is not None and _ints(work, "work", 0) < self.attn_work.numel():
             raise ValueError(f"work: {self.attn_work.numel()} ints")
         n = _ints(rows, "rows", 4)
-        self.lib.nsl_pages_attn(_stream(self.index), self._p, layer, _type(q), _ptr(q), qs, heads, hd ** -0.5 if scale is None else scale, window, _ptr(rows), n, max_rows, T,
+        stream = _stream(self.index)
+        if work is None:
+            work = self._work_of(stream)
+        self.lib.nsl_pages_attn(stream, self._p, layer, _type(q), _ptr(q), qs, heads, hd ** -0.5 if scale is None else scale, window, _ptr(rows), n, max_rows, T,
                                 _type(out, True), _ptr(out), os, _ptr(work))
         _done()
 

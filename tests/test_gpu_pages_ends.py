@@ -182,3 +182,67 @@ def test_attn_of_any_number_of_columns(cols, hd, page):
     pool.append(1, None, None, (k * grow ** 2).contiguous(), (torch.randn(n, 2, hd, generator=g, device="cuda")).contiguous(), ints([[0, n, 0, 0]]))
     q[::3] *= 0.01
     check_attn(pool, q.to(torch.bfloat16), [[0, cols, n - cols, 0]])
+
+
+# ---- calls beside one another -----------------------------------------------------------------------------------------------------------
+def calls_of(pool):
+    """Two calls whose items are all dealt to several blocks, so that both keep states in their work memory."""
+    g = gen_of(58)
+    out = []
+    for seqs in ([[0, 1, 2999, 0], [1, 1, 1999, 1]], [[0, 150, 2550, 0], [150, 3, 1900, 1]]):
+        q = torch.randn(153, 16, 128, generator=g, device="cuda").to(torch.bfloat16)
+        alone = torch.zeros_like(q)
+        rows, most = ints(seqs), max(n for _, n, _, _ in seqs)
+        pool.attn(1, q, rows, alone, max_rows=most)
+        out.append((q, rows, most, alone))
+    torch.cuda.synchronize()
+    return out
+
+
+def test_attn_on_two_streams_of_one_pool():
+    pool = random_pool(gen_of(59), 2, 700, 2, 128, 16, [3000, 2000])
+    calls = calls_of(pool)
+    streams = [torch.cuda.Stream() for _ in calls]
+    outs = [[torch.zeros_like(q) for _ in range(10)] for q, _, _, _ in calls]
+    torch.cuda.synchronize()
+    for i in range(10):
+        for (q, rows, most, _), stream, out in zip(calls, streams, outs):
+            with torch.cuda.stream(stream):
+                pool.attn(1, q, rows, out[i], max_rows=most)
+    torch.cuda.synchronize()
+    for (*_, alone), out in zip(calls, outs):
+        assert all(torch.equal(o, alone) for o in out)
+    handles = [s.cuda_stream for s in streams]
+    works = [pool._works[h].data_ptr() for h in handles]
+    assert len({*works, pool.attn_work.data_ptr()}) == 3
+    with torch.cuda.stream(streams[0]):      # the stream's own from then on
+        pool.attn(1, *calls[0][:2], outs[0][0], max_rows=calls[0][2])
+    assert pool._works[handles[0]].data_ptr() == works[0]
+    torch.cuda.synchronize()
+
+
+def test_attn_in_two_graphs_replayed_beside_one_another():
+    pool = random_pool(gen_of(59), 2, 700, 2, 128, 16, [3000, 2000])
+    calls = calls_of(pool)
+    graphs, outs, held_before = [], [], len(pool._works)
+    for q, rows, most, _ in calls:
+        out = torch.zeros_like(q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for layer in (0, 1, 0, 1):
+                pool.attn(layer, q, rows, out, max_rows=most)
+        graphs.append(graph)
+        outs.append(out)
+    assert len(pool._works) == held_before      # the memory is the graph's
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(10):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        pool.attn(1, calls[0][0], calls[0][1], torch.empty_like(outs[0]), max_rows=calls[0][2])      # and a call of the current stream's
+        torch.cuda.synchronize()
+        for out, (*_, alone) in zip(outs, calls):
+            assert torch.equal(out, alone)
