@@ -42,7 +42,8 @@ enum { NSL_ROPE_PLAIN = 0, NSL_ROPE_LINEAR = 1, NSL_ROPE_BASE = 2, NSL_ROPE_PART
 int nsl_rope_freqs(int kind, int rot, double theta, double scale, int ctx, double beta_fast, double beta_slow, float* inv, float* factor);
 /* Rows of heads rotated: x = factor (u cos a - w sin a, w cos a + u sin a), a = pos[t] * inv[p], the product reduced to a
  * quarter turn with all its bits (the angle is right to 1e-15 for every int32 position, its sine and cosine to 1.2e-10 and a rounding to f32).  q, qo [T][n_head][hd] with row strides in elements, k, ko [T][n_kv][hd]
- * (n_kv = 0: none; n_head = 0: none); outputs may be the inputs, and do not otherwise overlap them.  hd a multiple of 16, at
+ * (n_kv = 0: none; n_head = 0: none); outputs may be the inputs; a call whose outputs otherwise overlap
+ * them, or one another, is refused.  hd a multiple of 16, at
  * most 512; rows start on 16-byte boundaries. */
 void nsl_rope(cudaStream_t s, NslRope r, int type, int hd, const void* q, int q_stride, void* qo, int qo_stride, int n_head, const void* k, int k_stride,
               void* ko, int ko_stride, int n_kv, const int32_t* pos, int T);
@@ -65,7 +66,7 @@ typedef struct {
  * overlap.  Any int32 row and position may be named.  Rows that no descriptor names, or that lie outside [0, T), are left as they are. */
 typedef struct { int32_t row, rows, pos, seq; } NslSeqRows;
 
-/* Queries rotated (q -> qo, see nsl_rope; n_head = 0: none), keys rotated, and keys and values stored in the pages of layer
+/* Queries rotated (q -> qo, see nsl_rope; n_head = 0: none; a qo that overlaps k or v is refused), keys rotated, and keys and values stored in the pages of layer
  * `layer` that the sequences' table rows name (reserved before: nsl_pages_extend).  r.rot = 0: nothing is rotated.
  * A page's scale is a power of two, the smallest with max |x| <= 127 scale over what the page holds: it starts afresh with the
  * call that writes the page's first position and never shrinks until then; when a later row needs a larger one, the codes that
@@ -75,13 +76,13 @@ typedef struct { int32_t row, rows, pos, seq; } NslSeqRows;
 void nsl_pages_append(cudaStream_t s, const NslPages* p, int layer, NslRope r, int type, const void* q, int q_stride, void* qo, int qo_stride, int n_head,
                       const void* k, int k_stride, const void* v, int v_stride, const NslSeqRows* seqs, int n_seqs, int T);
 /* The values at the descriptors' positions -> ko, vo [T][n_kv][hd] (type NSL_F32: code * scale; the others: rounded to bf16).
- * Rows of positions without a page are left as they are. */
+ * Rows of positions without a page are left as they are; a ko that overlaps vo is refused. */
 void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void* ko, int ko_stride, void* vo, int vo_stride, const NslSeqRows* seqs, int n_seqs,
                     int T);
 
 /* Attention of each sequence's rows over its pages: the row at position P attends positions max(0, P - window + 1) .. P
  * (window <= 0: from 0) of its sequence, query head h over KV head h / (n_head / n_kv).  o = softmax(scale q.k) v, rounded to
- * bf16 (o_type NSL_BF16 or NSL_F32_BF16; o does not overlap q).  Positions without a page are left out, and so is what lies in a
+ * bf16 (o_type NSL_BF16 or NSL_F32_BF16; an o that overlaps q is refused).  Positions without a page are left out, and so is what lies in a
  * page behind the row's position, whatever it holds; a row that nothing is left for gives zeros.  Scales are not negative.  Here a
  * sequence may appear in several descriptors, and positions past 2^31 - 1 count as 2^31 - 1.
  * Queries take part with 11 significant bits (bf16 values exactly), weights with 11, sums in f32.

@@ -603,6 +603,12 @@ void nsl_pages_append(cudaStream_t s, const NslPages* p, int layer, NslRope r, i
         set_error("nsl_pages_append: layer %d of %d, type %d, %d rotated values of %d, no descriptors, or rows that are not 16-byte aligned", layer, p->n_layer, type, r.rot, p->hd);
         return;
     }
+    const int kw = p->n_kv * p->hd;
+    if (n_head && (!rows_same_or_apart(q, q_stride, qo, qo_stride, n_head * p->hd, type, T) || !rows_apart(qo, qo_stride, n_head * p->hd, type, k, k_stride, kw, type, T) ||
+                   !rows_apart(qo, qo_stride, n_head * p->hd, type, v, v_stride, kw, type, T))) {
+        set_error("nsl_pages_append: rotated queries that overlap the queries, keys or values");
+        return;
+    }
     FollowScope follow;
     AppendArgs a;
     a.p = *p; a.r = r; a.q = q; a.k = k; a.v = v; a.qo = qo; a.seqs = seqs;
@@ -635,6 +641,7 @@ void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void
         set_error("nsl_pages_read: layer %d of %d, type %d, no descriptors, or rows that are not 16-byte aligned", layer, p->n_layer, type);
         return;
     }
+    if (!rows_apart(ko, ko_stride, p->n_kv * p->hd, type, vo, vo_stride, p->n_kv * p->hd, type, T)) { set_error("nsl_pages_read: keys and values that overlap"); return; }
     FollowScope follow;
     int rows = 1;      // as many as leave four blocks an SM
     while (rows < READ_ROWS && T / (rows * 2) >= 4 * sm_count()) rows *= 2;

@@ -9,6 +9,19 @@ inline bool known_type(int t) { return t == NSL_F32 || t == NSL_BF16 || t == NSL
 inline int type_bytes(int t) { return t == NSL_BF16 ? 2 : 4; }
 // A row's base and stride: 16-byte steps, and room for the row.
 inline bool rows_ok(const void* p, int stride, int width, int type) { return p && aligned16(p) && stride >= width && ((size_t) stride * type_bytes(type)) % 16 == 0; }
+// Two arrays of T rows that have no byte in common: one lies behind the other, or their strides keep the rows beside one another.
+inline bool rows_apart(const void* a, int a_stride, int a_width, int a_type, const void* b, int b_stride, int b_width, int b_type, int T) {
+    const uint64_t at = (uint64_t) a, bt = (uint64_t) b, as = (uint64_t) a_stride * type_bytes(a_type), bs = (uint64_t) b_stride * type_bytes(b_type),
+                   aw = (uint64_t) a_width * type_bytes(a_type), bw = (uint64_t) b_width * type_bytes(b_type);
+    if (at + (T - 1) * as + aw <= bt || bt + (T - 1) * bs + bw <= at) return true;
+    uint64_t step = as;      // every distance between a row of a and one of b is bt - at and a multiple of this
+    for (uint64_t x = bs; x;) { const uint64_t r = step % x; step = x; x = r; }
+    const uint64_t d = bt >= at ? (bt - at) % step : (step - (at - bt) % step) % step;
+    return d >= aw && d + bw <= step;
+}
+inline bool rows_same_or_apart(const void* a, int a_stride, const void* b, int b_stride, int width, int type, int T) {
+    return (a == b && a_stride == b_stride) || rows_apart(a, a_stride, width, type, b, b_stride, width, type, T);
+}
 inline bool rope_ok(const NslRope& r, int hd) {
     return r.rot == 0 || (r.rot > 0 && r.rot % 16 == 0 && r.rot <= hd && r.inv && (r.layout == NSL_ROPE_HALF || r.layout == NSL_ROPE_INTERLEAVED));
 }

@@ -143,6 +143,7 @@ void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, co
                   q_type, o_type, n_head, p->n_kv, n_seqs);
         return;
     }
+    if (!rows_apart(q, q_stride, n_head * p->hd, q_type, o, o_stride, n_head * p->hd, o_type, T)) { set_error("nsl_pages_attn: results that overlap the queries"); return; }
     CUtensorMap tk, tv;
     if (!pattn_map(&tk, *p, p->k) || !pattn_map(&tv, *p, p->v)) { set_error("nsl_pages_attn: no tensor map for the pool's codes"); return; }
     FollowScope follow;

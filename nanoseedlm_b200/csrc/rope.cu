@@ -84,6 +84,13 @@ void nsl_rope(cudaStream_t s, NslRope r, int type, int hd, const void* q, int q_
         set_error("nsl_rope: type %d, %d + %d heads of %d values, %d of them rotated (a multiple of 16), no positions, or rows that are not 16-byte aligned", type, n_head, n_kv, hd, r.rot);
         return;
     }
+    const int qw = n_head * hd, kw = n_kv * hd;
+    if ((n_head && !rows_same_or_apart(q, q_stride, qo, qo_stride, qw, type, T)) || (n_kv && !rows_same_or_apart(k, k_stride, ko, ko_stride, kw, type, T)) ||
+        (n_head && n_kv && (!rows_apart(qo, qo_stride, qw, type, k, k_stride, kw, type, T) || !rows_apart(ko, ko_stride, kw, type, q, q_stride, qw, type, T) ||
+                            !rows_apart(qo, qo_stride, qw, type, ko, ko_stride, kw, type, T)))) {
+        set_error("nsl_rope: outputs that overlap the inputs or one another");
+        return;
+    }
     FollowScope follow;
     const unsigned grid = (unsigned) T;
     if (type == NSL_F32) launch(rope_kernel<NSL_F32>, grid, ROPE_THREADS, 0, s, r, hd, q, q_stride, qo, qo_stride, n_head, k, k_stride, ko, ko_stride, n_kv, pos);

@@ -246,3 +246,37 @@ def test_attn_in_two_graphs_replayed_beside_one_another():
         torch.cuda.synchronize()
         for out, (*_, alone) in zip(outs, calls):
             assert torch.equal(out, alone)
+
+
+# ---- outputs beside inputs ---------------------------------------------------------------------------------------------------------------
+def test_outputs_in_place_and_beside_the_inputs():
+    """Rows side by side in wider rows, behind one another, and in place are served; what overlaps is refused and nothing is written."""
+    g = gen_of(60)
+    pool = random_pool(g, 2, 30, 2, 64, 16, [100])
+    wide = torch.randn(9, 4 * 512, generator=g, device="cuda").to(torch.bfloat16)
+    cols = lambda i: wide[:, 512 * i:512 * i + 512].view(9, 8, 64)  # noqa: E731
+    q, seqs = cols(1), [[0, 9, 60, 0]]
+    want, size = attn64(pool, 1, q, seqs, 0.125, 0)
+    for out in (cols(0), cols(2), cols(3)):
+        pool.attn(1, q, ints(seqs), out, max_rows=9)
+        assert bool(((out.double() - want).abs() <= BF16 * want.abs() + (1 + BF16) * WEIGHTS * size).all())
+    behind = torch.zeros(18, 8, 64, dtype=torch.bfloat16, device="cuda")
+    behind[:9] = q
+    pool.attn(1, behind[:9], ints(seqs), behind[9:], max_rows=9)
+    assert torch.equal(behind[9:], cols(3)) and torch.equal(behind[:9], q)
+    keep, r, pos = wide.clone(), P().Rope(inv_of(64)), ints(list(range(9)))
+    k, v = torch.zeros(9, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(9, 2, 64, dtype=torch.bfloat16, device="cuda")
+    flat = wide.flatten()
+    part = lambda first: flat.as_strided((9, 8, 64), (2048, 64, 1), first)[:8]  # noqa: E731
+    bad = [lambda: pool.attn(1, q, ints(seqs), q, max_rows=9), lambda: pool.attn(1, q[:8], ints(seqs), part(512 + 8), max_rows=9), lambda: pool.attn(1, q[:8], ints(seqs), q[1:], max_rows=9),
+           lambda: P().rope(r, q[:8], None, pos[:8], part(512 + 64)), lambda: P().rope(r, q, cols(1)[:, :2], pos), lambda: P().rope(r, q, k, pos, cols(2), cols(2)[:, 4:6]),
+           lambda: pool.append(1, r, q, k, cols(2)[:, :2], ints(seqs), cols(2)), lambda: pool.read(1, ints(seqs), cols(0)[:, :2], cols(0)[:, 1:3])]
+    for call in bad:
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    assert torch.equal(wide, keep)
+    P().rope(r, q, cols(2), pos, cols(1), cols(3))      # in place, and beside
+    for a, b in ((1, 1), (2, 3)):
+        x = keep[:, 512 * a:512 * a + 512].view(9, 8, 64)
+        y, size = turned(x, pos, r.inv, False, 1.0)
+        assert bool(((cols(b).double() - y).abs() <= 4 * F32 * size + BF16 * (y.abs() + 4 * F32 * size)).all())

@@ -1,0 +1,47 @@
+"""More of what the paged cache's calls refuse on the host (nothing is launched, no GPU is needed)."""
+import ctypes as C
+
+import pytest
+from test_pages_host import A, pool, rope
+
+from nanoseedlm_b200 import lib as L
+
+
+def refused(why, fn, *args):
+    lib = L.load()
+    lib.nsl_last_error()
+    before = lib.nsl_launch_count()
+    getattr(lib, fn)(None, *args)
+    msg = L.last_error()
+    assert msg.startswith(fn) and why in msg, (msg, args)
+    assert lib.nsl_launch_count() == before
+
+
+# ---- outputs that overlap inputs or one another ----------------------------------------------------------------------------
+def at(byte):
+    return C.c_void_p(0x10000 + byte)
+
+
+W = 2 * 1024      # bytes of a row of 16 x 64 bf16 values
+OVERLAPS = [  # (output's first byte, its stride in values): inputs start at 0, 8 rows of 1024 bf16 values in rows of 4096 bytes
+    (16, 2048), (W - 16, 2048), (4096 - W + 16, 2048), (7 * 4096, 2048), (-7 * 4096, 2048), (0, 4096), (2 * 4096, 1024), (4096 * 3 + 2032, 2048), (W, 1536)]
+
+
+@pytest.mark.parametrize("byte,stride", OVERLAPS)
+def test_outputs_that_overlap(byte, stride):
+    p = C.byref(pool(hd=64, n_kv=16))
+    q = at(0x100000)
+    o = at(0x100000 + byte)
+    far = at(0x900000)
+    refused("overlap", "nsl_pages_attn", p, 0, 1, q, 2048, 16, 0.1, 0, A, 1, 4, 8, 1, o, stride, A)
+    refused("overlap", "nsl_rope", rope(rot=64), 1, 64, q, 2048, o, stride, 16, None, 0, None, 0, 0, A, 8)
+    refused("overlap", "nsl_rope", rope(rot=64), 1, 64, q, 2048, q, 2048, 16, far, 2048, o, stride, 16, A, 8)
+    refused("overlap", "nsl_rope", rope(rot=64), 1, 64, far, 2048, o, stride, 16, q, 2048, q, 2048, 16, A, 8)
+    refused("overlap", "nsl_pages_append", p, 0, rope(rot=64), 1, q, 2048, o, stride, 16, far, 2048, far, 2048, A, 1, 8)
+    refused("overlap", "nsl_pages_append", p, 0, rope(rot=64), 1, far, 2048, o, stride, 16, q, 2048, at(0xF00000), 2048, A, 1, 8)
+    refused("overlap", "nsl_pages_append", p, 0, rope(rot=64), 1, far, 2048, o, stride, 16, at(0xF00000), 2048, q, 2048, A, 1, 8)
+    refused("overlap", "nsl_pages_read", p, 0, 1, q, 2048, o, stride, A, 1, 8)
+
+
+def test_outputs_of_another_width_that_overlap():
+    refused("overlap", "nsl_pages_attn", C.byref(pool()), 0, 0, at(0), 2048, 16, 0.1, 0, A, 1, 4, 8, 1, at(4096), 2048, A)      # f32 rows of 8192 bytes, bf16 results within them
