@@ -6,7 +6,7 @@
  * KV head (value = code * scale), so the attention's products run on the codes and the scale is applied per page.
  *
  * Conventions as in nslm_kernels.h: the stream first, asynchronous launches that allocate nothing, the caller owns every
- * buffer; a call that is refused launches nothing and leaves a message in nsl_last_error().  Every kernel here waits on the
+ * buffer; a call that is refused launches nothing and leaves a message in nsl_last_error() and in nsl_pages_error().  Every kernel here waits on the
  * device for its predecessor before it reads anything and is a dependent launch unless nsl_dependent_launch(0) was called.
  * The tensors and the stream belong to the current device. */
 #pragma once
@@ -15,6 +15,10 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* Why this thread's last call of this header was refused, or "" if it was served.  nsl_last_error() keeps the first message that nobody has read,
+ * whatever call and thread it came from; one that is read here counts as read there too. */
+const char* nsl_pages_error(void);
 
 /* Elements of the queries, keys, values and results. */
 enum {

@@ -1,10 +1,12 @@
 // Host-side state of the library: the argument-error record, the launch counter, cached device properties and the
 // host stream table.  The product fails loudly: a call it cannot serve launches nothing and records why.
 #include "common.cuh"
+#include "../../include/nslm_pages.h"
 
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <cstring>
 #include <mutex>
 
 namespace nsl {
@@ -14,15 +16,19 @@ static std::mutex g_err_mu;
 static std::atomic<uint64_t> g_launches{0};
 thread_local int tl_pdl = PDL_OWN;
 
+static thread_local char tl_err[256];      // what this thread's present call was refused for (begin_call)
+
 void set_error(const char* fmt, ...) {
-    std::lock_guard<std::mutex> lk(g_err_mu);
-    if (g_err[0]) return;   // keep the first
     va_list ap;
     va_start(ap, fmt);
-    vsnprintf(g_err, sizeof g_err, fmt, ap);
+    vsnprintf(tl_err, sizeof tl_err, fmt, ap);
     va_end(ap);
+    std::lock_guard<std::mutex> lk(g_err_mu);
+    if (g_err[0]) return;   // keep the first
+    memcpy(g_err, tl_err, sizeof g_err);
     fprintf(stderr, "nslm_b200: %s\n", g_err);
 }
+void begin_call() { tl_err[0] = 0; }
 
 void count_launch(int n) { g_launches.fetch_add((uint64_t) n, std::memory_order_relaxed); }
 
@@ -54,6 +60,12 @@ const char* nsl_last_error(void) {
     snprintf(out, sizeof out, "%s", nsl::g_err);
     nsl::g_err[0] = 0;
     return out;
+}
+
+const char* nsl_pages_error(void) {
+    std::lock_guard<std::mutex> lk(nsl::g_err_mu);
+    if (nsl::tl_err[0] && !strcmp(nsl::tl_err, nsl::g_err)) nsl::g_err[0] = 0;
+    return nsl::tl_err;
 }
 
 uint64_t nsl_launch_count(void) { return nsl::g_launches.load(std::memory_order_relaxed); }

@@ -8,6 +8,7 @@
 namespace nsl {
 
 void set_error(const char* fmt, ...);
+void begin_call();      // forgets what this thread's last call was refused for (nsl_pages_error)
 void count_launch(int n = 1);
 int sm_count();
 int max_smem_optin();

@@ -596,6 +596,7 @@ extern "C" {
 
 void nsl_pages_append(cudaStream_t s, const NslPages* p, int layer, NslRope r, int type, const void* q, int q_stride, void* qo, int qo_stride, int n_head,
                       const void* k, int k_stride, const void* v, int v_stride, const NslSeqRows* seqs, int n_seqs, int T) {
+    begin_call();
     if (T <= 0 || n_seqs <= 0) return;
     if (!pages_ok(p, "nsl_pages_append")) return;
     if (!layer_ok(p, layer) || !known_type(type) || !rope_ok(r, p->hd) || !seqs || n_head < 0 || n_head > 65536 || (n_head && (!rows_ok(q, q_stride, n_head * p->hd, type) || !rows_ok(qo, qo_stride, n_head * p->hd, type))) ||
@@ -635,6 +636,7 @@ void nsl_pages_append(cudaStream_t s, const NslPages* p, int layer, NslRope r, i
 }
 
 void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void* ko, int ko_stride, void* vo, int vo_stride, const NslSeqRows* seqs, int n_seqs, int T) {
+    begin_call();
     if (T <= 0 || n_seqs <= 0) return;
     if (!pages_ok(p, "nsl_pages_read")) return;
     if (!layer_ok(p, layer) || !known_type(type) || !seqs || !rows_ok(ko, ko_stride, p->n_kv * p->hd, type) || !rows_ok(vo, vo_stride, p->n_kv * p->hd, type)) {
@@ -653,6 +655,7 @@ void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void
 }
 
 void nsl_pages_extend(cudaStream_t s, const NslPages* p, const NslPagesLen* reqs, int n, int32_t* got) {
+    begin_call();
     if (n <= 0 || !pages_ok(p, "nsl_pages_extend") || !list_ok(reqs, n, "nsl_pages_extend")) return;
     FollowScope follow;
     launch(extend_kernel, 1, MAN_THREADS, 0, s, *p, reqs, n, got);
@@ -661,6 +664,7 @@ void nsl_pages_extend(cudaStream_t s, const NslPages* p, const NslPagesLen* reqs
 }
 
 void nsl_pages_fork(cudaStream_t s, const NslPages* p, const NslPagesFork* forks, int n) {
+    begin_call();
     if (n <= 0 || !pages_ok(p, "nsl_pages_fork") || !list_ok(forks, n, "nsl_pages_fork")) return;
     FollowScope follow;
     launch(fork_kernel, 1, MAN_THREADS, 0, s, *p, forks, n);
@@ -668,6 +672,7 @@ void nsl_pages_fork(cudaStream_t s, const NslPages* p, const NslPagesFork* forks
 }
 
 void nsl_pages_trim(cudaStream_t s, const NslPages* p, const NslPagesLen* reqs, int n) {
+    begin_call();
     if (n <= 0 || !pages_ok(p, "nsl_pages_trim") || !list_ok(reqs, n, "nsl_pages_trim")) return;
     FollowScope follow;
     launch(trim_kernel, 1, MAN_THREADS, 0, s, *p, reqs, n);
@@ -675,6 +680,7 @@ void nsl_pages_trim(cudaStream_t s, const NslPages* p, const NslPagesLen* reqs, 
 }
 
 void nsl_pages_compact(cudaStream_t s, const NslPages* p) {
+    begin_call();
     if (!pages_ok(p, "nsl_pages_compact")) return;
     FollowScope follow;
     launch(compact_kernel, 1, MAN_THREADS, 0, s, *p);
@@ -683,6 +689,7 @@ void nsl_pages_compact(cudaStream_t s, const NslPages* p) {
 }
 
 void nsl_pages_copy(cudaStream_t s, const NslPages* p, const int32_t* pairs, int n) {
+    begin_call();
     if (n <= 0 || !pages_ok(p, "nsl_pages_copy")) return;
     if (!pairs) { set_error("nsl_pages_copy: no list"); return; }
     FollowScope follow;

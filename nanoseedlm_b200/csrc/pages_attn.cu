@@ -126,6 +126,7 @@ extern "C" {
 size_t nsl_pages_attn_work(void) { return (size_t) pattn_blocks() * 16 + (size_t) sm_count() * 2 * PATTN_MANY * PATTN_STATE<128> * 4; }
 
 int nsl_pages_attn_status(void) {
+    begin_call();
     const int few = pattn_few_status();
     return few ? few : pattn_many_status();
 }
@@ -135,6 +136,7 @@ void nsl_pages_attn_hold(unsigned long long wait_ns) { tl_hold_ns = wait_ns < PA
 
 void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, const void* q, int q_stride, int n_head, float scale, int window,
                     const NslSeqRows* seqs, int n_seqs, int max_rows, int T, int o_type, void* o, int o_stride, void* work) {
+    begin_call();
     if (T <= 0 || n_seqs <= 0 || max_rows <= 0) return;
     if (!pages_ok(p, "nsl_pages_attn")) return;
     if (!layer_ok(p, layer) || !known_type(q_type) || (o_type != NSL_BF16 && o_type != NSL_F32_BF16) || n_head < 1 || n_head % p->n_kv || n_head > 65535 || (long long) n_head * T > 0x7FFFFFFF || !seqs || n_seqs > 4096 ||

@@ -46,6 +46,7 @@ using namespace nsl;
 extern "C" {
 
 int nsl_rope_freqs(int kind, int rot, double theta, double scale, int ctx, double beta_fast, double beta_slow, float* inv, float* factor) {
+    begin_call();
     if (kind < NSL_ROPE_PLAIN || kind > NSL_ROPE_PARTS || rot < 2 || rot % 2 || !(theta > 1.0) || !(scale >= 1.0) || !inv || !factor || (kind == NSL_ROPE_BASE && rot < 4) ||
         (kind == NSL_ROPE_PARTS && (ctx < 1 || !(beta_fast > beta_slow) || !(beta_slow > 0.0)))) {
         set_error("nsl_rope_freqs: kind %d, %d rotated values, theta %g, scale %g, %d positions, betas %g and %g", kind, rot, theta, scale, ctx, beta_fast, beta_slow);
@@ -77,6 +78,7 @@ int nsl_rope_freqs(int kind, int rot, double theta, double scale, int ctx, doubl
 
 void nsl_rope(cudaStream_t s, NslRope r, int type, int hd, const void* q, int q_stride, void* qo, int qo_stride, int n_head, const void* k, int k_stride,
               void* ko, int ko_stride, int n_kv, const int32_t* pos, int T) {
+    begin_call();
     if (T <= 0) return;
     if (!known_type(type) || hd < 16 || hd % 16 || hd > 2 * ROPE_MAX_PAIRS || n_head < 0 || n_kv < 0 || (n_head > 0) + (n_kv > 0) == 0 || (long long) (n_head + n_kv) * hd > (1 << 24) ||
         r.rot == 0 || !rope_ok(r, hd) || !pos || (n_head && (!rows_ok(q, q_stride, n_head * hd, type) || !rows_ok(qo, qo_stride, n_head * hd, type))) ||

@@ -204,6 +204,7 @@ PROTOTYPES = {
     "nsl_xcache_stats": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
     "nsl_xcache_set_ops": (None, [_vp]),
     # include/nslm_pages.h
+    "nsl_pages_error": (C.c_char_p, []),
     "nsl_rope_freqs": (_i, [_i, _i, C.c_double, C.c_double, _i, C.c_double, C.c_double, _vp, _vp]),
     "nsl_rope": (None, [_vp, NslRope, _i, _i, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _i, _vp, _i]),
     "nsl_pages_append": (None, [_vp, _vp, _i, NslRope, _i, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _i]),

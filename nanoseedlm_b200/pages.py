@@ -16,7 +16,7 @@ def rope_freqs(rot, theta, kind=ROPE_PLAIN, scale=1.0, ctx=0, beta_fast=32.0, be
     """-> (frequencies float32 [rot / 2] on the host, factor): see nsl_rope_freqs."""
     inv, factor = np.zeros(max(rot // 2, 1), np.float32), C.c_float()
     if L.load().nsl_rope_freqs(kind, rot, theta, scale, ctx, beta_fast, beta_slow, C.c_void_p(inv.ctypes.data), C.byref(factor)):
-        raise ValueError(L.last_error())
+        _done()
     return inv, factor.value
 
 
@@ -77,8 +77,8 @@ def _here(index, *tensors):
 
 
 def _done():
-    """Raises what the call was refused for."""
-    msg = L.load().nsl_last_error()
+    """Raises what this thread's last call was refused for."""
+    msg = L.load().nsl_pages_error()
     if msg:
         raise ValueError(msg.decode())
 
@@ -218,7 +218,7 @@ class PagePool:
         with torch.cuda.device(self.device):
             code = self.lib.nsl_pages_attn_status()
         if code < 0:
-            raise RuntimeError(L.last_error() or "nsl_pages_attn_status failed")
+            raise RuntimeError(self.lib.nsl_pages_error().decode())
         return code
 
     def extend(self, reqs, got=None):

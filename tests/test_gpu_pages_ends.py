@@ -2,6 +2,7 @@
 
 Roundings that the tolerances count (half a step each, relative): f32 2^-24, bf16 2^-8, f16 2^-11."""
 import math
+import threading
 from fractions import Fraction
 
 import pytest
@@ -280,3 +281,21 @@ def test_outputs_in_place_and_beside_the_inputs():
         x = keep[:, 512 * a:512 * a + 512].view(9, 8, 64)
         y, size = turned(x, pos, r.inv, False, 1.0)
         assert bool(((cols(b).double() - y).abs() <= 4 * F32 * size + BF16 * (y.abs() + 4 * F32 * size)).all())
+
+
+# ---- whose refusal the handle raises -------------------------------------------------------------------------------------------------------
+def test_a_served_call_raises_nothing():
+    """Refusals that nobody has read, of this thread's other calls and of another thread's, are not the handle's."""
+    lib, pool = P().L.load(), P().PagePool.empty(1, 8, 1, 64, 16, 2, 4)
+    bad = lambda: lib.nsl_pages_fork(None, pool._p, None, 1)  # noqa: E731
+    bad()
+    t = threading.Thread(target=bad)
+    t.start()
+    t.join()
+    x, rows = torch.randn(3, 1, 64, device="cuda"), ints([[0, 3, 0, 0]])
+    pool.extend(ints([[0, 3]]))
+    pool.append(0, None, None, x, x, rows)
+    pool.attn(0, x, rows, torch.empty_like(x), max_rows=3)
+    with pytest.raises(ValueError, match="nsl_pages_append"):
+        pool.append(1, None, None, x, x, rows)
+    assert P().L.last_error().startswith("nsl_pages_fork")

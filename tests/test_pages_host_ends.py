@@ -1,10 +1,12 @@
 """More of what the paged cache's calls refuse on the host (nothing is launched, no GPU is needed)."""
 import ctypes as C
+import threading
 
 import pytest
 from test_pages_host import A, pool, rope
 
 from nanoseedlm_b200 import lib as L
+from nanoseedlm_b200 import pages as P
 
 
 def refused(why, fn, *args):
@@ -45,3 +47,31 @@ def test_outputs_that_overlap(byte, stride):
 
 def test_outputs_of_another_width_that_overlap():
     refused("overlap", "nsl_pages_attn", C.byref(pool()), 0, 0, at(0), 2048, 16, 0.1, 0, A, 1, 4, 8, 1, at(4096), 2048, A)      # f32 rows of 8192 bytes, bf16 results within them
+
+
+# ---- whose refusal a call reports -------------------------------------------------------------------------------------------------
+def test_a_call_reports_its_own_refusal_only():
+    lib, p = L.load(), C.byref(pool())
+    lib.nsl_last_error()
+    lib.nsl_pages_fork(None, p, None, 1)      # refused, and not read
+    lib.nsl_pages_copy(None, p, A, 0)         # an empty call
+    assert lib.nsl_pages_error() == b""
+    with pytest.raises(ValueError, match="nsl_rope_freqs"):
+        P.rope_freqs(63, 1e4)
+    P.rope_freqs(64, 1e4)
+    assert lib.nsl_pages_error() == b""
+    assert L.last_error().startswith("nsl_pages_fork") and L.last_error() == ""
+    lib.nsl_pages_trim(None, p, None, 1)
+    assert lib.nsl_pages_error().startswith(b"nsl_pages_trim") and L.last_error() == ""      # read here, read there
+
+
+def test_a_call_reports_nothing_of_other_threads():
+    lib, p = L.load(), C.byref(pool())
+    lib.nsl_last_error()
+    lib.nsl_pages_copy(None, p, A, 0)
+    seen = []
+    t = threading.Thread(target=lambda: (lib.nsl_pages_fork(None, p, None, 1), seen.append(lib.nsl_pages_error())))
+    t.start()
+    t.join()
+    assert seen[0].startswith(b"nsl_pages_fork") and lib.nsl_pages_error() == b""
+    lib.nsl_last_error()
