@@ -299,3 +299,90 @@ def test_a_served_call_raises_nothing():
     with pytest.raises(ValueError, match="nsl_pages_append"):
         pool.append(1, None, None, x, x, rows)
     assert P().L.last_error().startswith("nsl_pages_fork")
+
+
+# ---- queries that are not finite ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,heads,hd,page", [(1, 8, 128, 64), (2, 8, 64, 16), (5, 8, 128, 16), (40, 8, 64, 64), (300, 4, 128, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_attn_of_queries_that_are_not_finite(rows, heads, hd, page, dtype, what):
+    """The softmax of scores that hold a NaN, or an infinity times codes of both signs and 0, is NaN: so is that row's head, and nothing else; a row that
+    nothing is left for gives zeros whatever its query holds."""
+    g = gen_of(54)
+    pool = random_pool(g, 2, 80, 2, hd, page, [900, 64])
+    q = torch.randn(rows + 1, heads, hd, generator=g, device="cuda").to(torch.bfloat16).to(dtype)
+    seqs = [[0, rows, 899 - rows, 0], [rows, 1, -4, 1]]
+    a = check_attn(pool, q, seqs, out_dtype=dtype)
+    bad = q.clone()
+    bad[rows // 2, 1, 7] = what
+    bad[rows, 0, 3] = what
+    b = torch.full_like(a, 5.0)
+    pool.attn(1, bad, ints(seqs), b, max_rows=rows)
+    assert bool(b[rows // 2, 1].isnan().all()) and bool((b[rows] == 0).all())
+    b[rows // 2, 1] = a[rows // 2, 1]
+    assert torch.equal(a, b)
+
+
+# ---- page scales far apart, masked pages and large pools, on both attention kernels and all page sizes ---------------------------------
+FORMS = [(1, 4, 128, 64), (1, 4, 64, 16), (2, 4, 64, 128), (1, 8, 128, 16), (2, 2, 128, 128), (3, 8, 128, 64), (5, 8, 64, 128), (200, 4, 128, 128), (150, 2, 64, 64), (100, 8, 64, 32)]      # rows, heads a KV head, hd, page
+
+
+@pytest.mark.parametrize("rows,group,hd,page", FORMS, ids=str)
+def test_attn_scales_far_apart(rows, group, hd, page):
+    g = gen_of(13 + rows + page)
+    pool = random_pool(g, 2, 2 * (-(-700 // page)) + 3, 2, hd, page, [700, 300])
+    pool.vs.copy_(torch.exp2(torch.randint(-60, 40, pool.vs.shape, generator=g, device="cuda").float()))
+    pool.ks[:, ::5] = 0.0
+    pool.vs[:, ::7] = 0.0
+    q = torch.randn(2 * rows, 2 * group, hd, generator=g, device="cuda").to(torch.bfloat16)
+    seqs = [[0, rows, 700 - rows, 0], [rows, rows, 250 - rows, 1]]
+    check_attn(pool, q, seqs, scale=0.01)
+    check_attn(pool, q, seqs, scale=0.01, window=page + 3)
+    check_attn(pool, q * 0, seqs)
+    pool.vs.copy_(torch.exp2(torch.arange(pool.vs.numel(), device="cuda").view(pool.vs.shape) % 120 - 110.0))      # up to 2^119 between neighbours
+    check_attn(pool, q, seqs, scale=0.01)
+    pool.vs.fill_(0.0)
+    assert bool((check_attn(pool, q, seqs) == 0).all())
+
+
+@pytest.mark.parametrize("rows,group,hd,page", FORMS, ids=str)
+def test_attn_takes_nothing_from_masked_pages(rows, group, hd, page):
+    """Scales and codes of pages outside the window or behind the last position may be anything."""
+    g = gen_of(14 + rows + page)
+    pool = random_pool(g, 2, 2 * (-(-1400 // page)) + 3, 2, hd, page, [1400, 1400])
+    q = torch.randn(2 * rows, 2 * group, hd, generator=g, device="cuda").to(torch.bfloat16)
+    at = 1000 // page * page - 1      # the last row's position is the last of its page
+    seqs = [[0, rows, at - rows + 1, 0], [rows, rows, 700 - rows, 1]]
+    a = check_attn(pool, q, seqs, window=100)
+    dead = [pool.table[0, (at + 1) // page:], pool.table[1, 700 // page + 1:], pool.table[0, :(at - rows - 100) // page], pool.table[1, :max(0, 700 - rows - 100) // page]]
+    for n, ids in enumerate(dead):
+        for t in (pool.ks, pool.vs):
+            t[:, ids.long()] = [float("nan"), float("inf"), -1.0, 0.0][n]
+        pool.k[:, ids.long()] = 127
+        pool.v[:, ids.long()] = -128
+    b = check_attn(pool, q, seqs, window=100)
+    assert torch.equal(a, b)
+    # codes behind the last position, in its own page
+    pool.k[:, pool.table[1, 700 // page].long(), :, 700 % page:] = 127
+    pool.v[:, pool.table[1, 700 // page].long(), :, 700 % page:] = -127
+    assert torch.equal(a, check_attn(pool, q, seqs, window=100))
+
+
+@pytest.mark.parametrize("hd,page", [(128, 64), (128, 16), (64, 128)])
+def test_attn_of_single_rows_beyond_32_bits(hd, page):
+    """Pages more than 2^32 bytes into the pool, read by the kernel of few columns."""
+    kv = 8
+    pages = (1 << 32) // (kv * hd * page) + 2000
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 20 GB")
+    shape = (1, pages, kv, page, hd)
+    k, v = (torch.empty(shape, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.full(shape[:3], 2.0 ** -6, device="cuda") for _ in range(2))
+    g = gen_of(16)
+    ids = [pages - 1, 3, pages - 2, 7, pages - 1900]
+    for i in ids:
+        for t in (k, v):
+            t[0, i] = torch.randint(-127, 128, shape[2:], generator=g, device="cuda", dtype=torch.int32).to(torch.int8)
+    pool = P().PagePool(k, v, ks, vs, torch.ones(pages, dtype=torch.int32, device="cuda"), ints([ids, ids[::-1]]), ints([5 * page] * 2))
+    q = torch.randn(2, 16, hd, generator=g, device="cuda").to(torch.bfloat16)
+    check_attn(pool, q, [[0, 1, 5 * page - 1, 0], [1, 1, 3 * page + 2, 1]], layer=0)
