@@ -24,7 +24,7 @@ const char* nsl_pages_error(void);
 enum {
     NSL_F32 = 0,          /* f32, results unrounded */
     NSL_BF16 = 1,         /* packed bf16 */
-    NSL_F32_BF16 = 2      /* f32 arrays whose results are rounded to bf16 (the engine's activations) */
+    NSL_F32_BF16 = 2      /* f32 arrays of bf16 values: results are rounded to bf16 (the engine's activations) */
 };
 
 /* ---- rotary positions --------------------------------------------------------------------------------------------------- */
@@ -89,7 +89,9 @@ void nsl_pages_read(cudaStream_t s, const NslPages* p, int layer, int type, void
  * bf16 (o_type NSL_BF16 or NSL_F32_BF16; an o that overlaps q is refused).  Positions without a page are left out, and so is what lies in a
  * page behind the row's position, whatever it holds; a row that nothing is left for gives zeros.  Scales are not negative.  Here a
  * sequence may appear in several descriptors, and positions past 2^31 - 1 count as 2^31 - 1.
- * Queries take part with 11 significant bits (bf16 values exactly), weights with 11, sums in f32.
+ * Queries are held as f16 after their head's largest magnitude's power of two is divided out (bf16 values exactly, elements below 2^-17 of
+ * the largest to 2^-25 of it), for q_type NSL_F32 as two such terms (22 bits, or 2^-25 of the largest); q_type NSL_F32_BF16 says that the values
+ * are bf16's, and one term is taken.  Weights times their page's value scale are held as f16 too (11 bits, or 2^-25 of the largest of the row); sums in f32.
  * max_rows: no descriptor has more rows (rows beyond it are left as they are).  work: nsl_pages_attn_work() bytes of device
  * memory (40 MB for 148 multiprocessors), 16-byte aligned, no initial contents; calls that share it run one behind the other, captured ones too.
  * The step's keys are dealt evenly to the blocks, so a row alone and in a batch may differ in the order of its f32 sums; a call

@@ -90,6 +90,12 @@ __device__ __forceinline__ uint32_t pa_f16x2(float lo, float hi) {      // round
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// What x and y lost when they were rounded to the f16 pair `rounded`, rounded to f16 themselves.
+__device__ __forceinline__ uint32_t pa_low_f16x2(float x, float y, uint32_t rounded) {
+    float lo, hi;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(lo), "=f"(hi) : "r"(rounded));
+    return pa_f16x2(x - lo, y - hi);
+}
 // Two bytes (signed codes ^ 0x80, picked by SEL from x) as two f16 values: a byte u under the exponent of 1024 is 1024 + u, and
 // 1024 + (code + 128) - 1152 is the code, exactly.
 template <uint32_t SEL>

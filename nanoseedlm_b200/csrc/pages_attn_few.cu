@@ -8,12 +8,15 @@
 // a ring.  Four warps compute, 16 keys of the unit each, on the tensor cores with the codes as they are:
 //   S^T [16 keys][8 columns]     = K [16 keys][hd] . Q^T       A = codes by ldmatrix (a lane's 4 bytes are 4 dims of a key)
 //   O^T [16 dims][8 columns]    += V^T [dims][16 keys] . W^T   A = codes by ldmatrix.trans (2 dims of 2 keys)
+// Queries of f32 calls whose rounding to f16 leaves something off take part with that as a second f16 term, by the same code fragments.
 // A code becomes f16 by a byte permutation and a subtraction (exact); a page's key scale multiplies the scores, its value
 // scale is part of the weights' exponent: w = 2^(s + log2 vs - mo), mo the running maximum of that sum, beside the softmax's own
 // p = 2^(s - m) whose sum is l.  Weights then never exceed 1 however the pages' scales differ, and 11 bits of f16 are 11
 // bits of each weight.  result = O 2^(mo - m) / l.
 // A run that ends inside an item (sequence, KV head) leaves its state in the work memory; the merge kernel (pages_attn.cu), a
 // dependent launch, joins an item's states in the order of the keys.
+#include <type_traits>
+
 #include "pages_attn.cuh"
 
 namespace nsl {
@@ -113,7 +116,8 @@ __device__ __forceinline__ void few_weights(const float* p, int c, float* cw, fl
     of_all[3 * c] = m; of_all[3 * c + 1] = l; of_all[3 * c + 2] = mo;
 }
 
-template <int HD>
+// FINE: f32 calls, whose queries may have second terms.
+template <int HD, bool FINE>
 __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
     using F = Few<HD>;
     constexpr int CT = F::CT, STATE = F::STATE, STEPS = HD / 16;
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
     while (walk.next(a, group, x, xe, &it)) {
         const int cols = it.sp.rows * group;
         // the queries as B fragments: column r0 of a tile, dims 16 j + 4 q4 ..; a column divided by its power of two
-        uint32_t qb[STEPS][2];
+        uint32_t qb[STEPS][2], ql[STEPS][2], some = 0;      // ql: what the rounding to f16 left off, as f16 again; low: any of it is not 0
         float f[2];      // of the lane's columns 2 q4, 2 q4 + 1: scale, log2 e and the power of two
         int hi[2], lo[2];
         const int c = r0;
@@ -257,7 +261,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
         for (int j = 0; j < STEPS; ++j) {
             qb[j][0] = pa_f16x2(v[j][0] * inv, v[j][1] * inv);
             qb[j][1] = pa_f16x2(v[j][2] * inv, v[j][3] * inv);
+            if (FINE) {
+                ql[j][0] = pa_low_f16x2(v[j][0] * inv, v[j][1] * inv, qb[j][0]);
+                ql[j][1] = pa_low_f16x2(v[j][2] * inv, v[j][3] * inv, qb[j][1]);
+                some |= ql[j][0] | ql[j][1];
+            }
         }
+        const bool low = FINE && __any_sync(0xFFFFFFFFu, (some & 0x7FFF7FFFu) != 0);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             f[e] = __shfl_sync(0xFFFFFFFFu, fc, 4 * (2 * q4 + e));
@@ -270,75 +280,82 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
         l[0] = l[1] = 0.0f;
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) ot[i][0] = ot[i][1] = ot[i][2] = ot[i][3] = 0.0f;
-        for (x = it.x0; x < it.x1; ++x) {
-            wait(full + 8 * stage, round & 1, 2);
-            const float4 mt = meta[4 * stage + warp];
-            const int key = (it.tile0 + x - it.first) * FEW_KEYS + 16 * warp;
-            if (mt.z != 0.0f && key < it.k1 && key + 16 > it.k0) {
-                const uint32_t kt = ring + stage * 2 * F::TILE + l_at;
-                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // two chains
+        // the item's units; LOW: with the second terms (a loop of its own: a branch in one loop for both cost the calls without them 4 %)
+        auto attend = [&](auto with_low) {
+            constexpr bool LOW = decltype(with_low)::value;
+            for (x = it.x0; x < it.x1; ++x) {
+                wait(full + 8 * stage, round & 1, 2);
+                const float4 mt = meta[4 * stage + warp];
+                const int key = (it.tile0 + x - it.first) * FEW_KEYS + 16 * warp;
+                if (mt.z != 0.0f && key < it.k1 && key + 16 > it.k0) {
+                    const uint32_t kt = ring + stage * 2 * F::TILE + l_at;
+                    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // two chains
 #pragma unroll
-                for (int j = 0; j < STEPS; j += 2) {
-                    uint32_t c[4];
-                    few_ldsm(c, kt + ((l_x ^ (uint32_t) j) << 4));
+                    for (int j = 0; j < STEPS; j += 2) {
+                        uint32_t c[4];
+                        few_ldsm(c, kt + ((l_x ^ (uint32_t) j) << 4));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) c[e] ^= 0x80808080u;
-                    const uint32_t a0[4] = {pa_codes<0x4140>(c[0]), pa_codes<0x4140>(c[1]), pa_codes<0x4342>(c[0]), pa_codes<0x4342>(c[1])};
-                    const uint32_t a1[4] = {pa_codes<0x4140>(c[2]), pa_codes<0x4140>(c[3]), pa_codes<0x4342>(c[2]), pa_codes<0x4342>(c[3])};
-                    few_mma(s, a0, qb[j]);
-                    few_mma(s2, a1, qb[j + 1]);
+                        for (int e = 0; e < 4; ++e) c[e] ^= 0x80808080u;
+                        const uint32_t a0[4] = {pa_codes<0x4140>(c[0]), pa_codes<0x4140>(c[1]), pa_codes<0x4342>(c[0]), pa_codes<0x4342>(c[1])};
+                        const uint32_t a1[4] = {pa_codes<0x4140>(c[2]), pa_codes<0x4140>(c[3]), pa_codes<0x4342>(c[2]), pa_codes<0x4342>(c[3])};
+                        few_mma(s, a0, qb[j]);
+                        few_mma(s2, a1, qb[j + 1]);
+                        if (LOW) { few_mma(s, a0, ql[j]); few_mma(s2, a1, ql[j + 1]); }
+                    }
+                    uint32_t pw[2];
+                    float mx[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {      // keys key + r0 and key + r0 + 8 of column 2 q4 + e
+                        const float fk = f[e] * mt.x;
+                        const int ka = key + r0, kb = ka + 8;
+                        s[e] = ka <= hi[e] && ka >= lo[e] ? (s[e] + s2[e]) * fk : -INFINITY;
+                        s[2 + e] = kb <= hi[e] && kb >= lo[e] ? (s[2 + e] + s2[2 + e]) * fk : -INFINITY;
+                        mx[e] = fmaxf(s[e], s[2 + e]);
+                    }
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xFFFFFFFFu, mx[0], o));
+                        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xFFFFFFFFu, mx[1], o));
+                    }
+                    float cor[2], w[4];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float mn = fmaxf(m[e], mx[e]), ms = mn == -INFINITY ? 0.0f : mn;
+                        const float mon = fmaxf(mo[e], mx[e] + mt.y), mos = mon == -INFINITY ? 0.0f : mon;
+                        l[e] = fmaf(l[e], pa_ex2(m[e] - ms), pa_ex2(s[e] - ms) + pa_ex2(s[2 + e] - ms));
+                        cor[e] = pa_ex2(mo[e] - mos);
+                        w[e] = s[e] == -INFINITY ? 0.0f : pa_ex2(s[e] + (mt.y - mos));      // (an infinite scale counts for those who attend its page)
+                        w[2 + e] = s[2 + e] == -INFINITY ? 0.0f : pa_ex2(s[2 + e] + (mt.y - mos));
+                        m[e] = mn;
+                        mo[e] = mon;
+                    }
+                    if (cor[0] != 1.0f || cor[1] != 1.0f) {      // the running maxima rarely move after a run's first steps
+#pragma unroll
+                        for (int i = 0; i < STEPS; ++i) { ot[i][0] *= cor[0]; ot[i][1] *= cor[1]; ot[i][2] *= cor[0]; ot[i][3] *= cor[1]; }
+                    }
+                    __syncwarp();      // lanes that had a maximum move and lanes that had none: what follows is the whole warp's
+                    pw[0] = few_turn(pa_f16x2(w[0], w[1]));
+                    pw[1] = few_turn(pa_f16x2(w[2], w[3]));
+#pragma unroll
+                    for (int j = 0; j < STEPS; j += 2) {
+                        uint32_t c[4];
+                        few_ldsm_trans(c, kt + F::TILE + ((l_x ^ (uint32_t) j) << 4));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[e] ^= 0x80808080u;
+                        // row r0 of value tile j: dim 16 j + 2 r0, row r0 + 8: the next
+                        const uint32_t a0[4] = {pa_codes<0x4240>(c[0]), pa_codes<0x4341>(c[0]), pa_codes<0x4240>(c[1]), pa_codes<0x4341>(c[1])};
+                        const uint32_t a1[4] = {pa_codes<0x4240>(c[2]), pa_codes<0x4341>(c[2]), pa_codes<0x4240>(c[3]), pa_codes<0x4341>(c[3])};
+                        few_mma(ot[j], a0, pw);
+                        few_mma(ot[j + 1], a1, pw);
+                    }
                 }
-                uint32_t pw[2];
-                float mx[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {      // keys key + r0 and key + r0 + 8 of column 2 q4 + e
-                    const float fk = f[e] * mt.x;
-                    const int ka = key + r0, kb = ka + 8;
-                    s[e] = ka <= hi[e] && ka >= lo[e] ? (s[e] + s2[e]) * fk : -INFINITY;
-                    s[2 + e] = kb <= hi[e] && kb >= lo[e] ? (s[2 + e] + s2[2 + e]) * fk : -INFINITY;
-                    mx[e] = fmaxf(s[e], s[2 + e]);
-                }
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) {
-                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xFFFFFFFFu, mx[0], o));
-                    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xFFFFFFFFu, mx[1], o));
-                }
-                float cor[2], w[4];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float mn = fmaxf(m[e], mx[e]), ms = mn == -INFINITY ? 0.0f : mn;
-                    const float mon = fmaxf(mo[e], mx[e] + mt.y), mos = mon == -INFINITY ? 0.0f : mon;
-                    l[e] = fmaf(l[e], pa_ex2(m[e] - ms), pa_ex2(s[e] - ms) + pa_ex2(s[2 + e] - ms));
-                    cor[e] = pa_ex2(mo[e] - mos);
-                    w[e] = s[e] == -INFINITY ? 0.0f : pa_ex2(s[e] + (mt.y - mos));      // (an infinite scale counts for those who attend its page)
-                    w[2 + e] = s[2 + e] == -INFINITY ? 0.0f : pa_ex2(s[2 + e] + (mt.y - mos));
-                    m[e] = mn;
-                    mo[e] = mon;
-                }
-                if (cor[0] != 1.0f || cor[1] != 1.0f) {      // the running maxima rarely move after a run's first steps
-#pragma unroll
-                    for (int i = 0; i < STEPS; ++i) { ot[i][0] *= cor[0]; ot[i][1] *= cor[1]; ot[i][2] *= cor[0]; ot[i][3] *= cor[1]; }
-                }
-                __syncwarp();      // lanes that had a maximum move and lanes that had none: what follows is the whole warp's
-                pw[0] = few_turn(pa_f16x2(w[0], w[1]));
-                pw[1] = few_turn(pa_f16x2(w[2], w[3]));
-#pragma unroll
-                for (int j = 0; j < STEPS; j += 2) {
-                    uint32_t c[4];
-                    few_ldsm_trans(c, kt + F::TILE + ((l_x ^ (uint32_t) j) << 4));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) c[e] ^= 0x80808080u;
-                    // row r0 of value tile j: dim 16 j + 2 r0, row r0 + 8: the next
-                    const uint32_t a0[4] = {pa_codes<0x4240>(c[0]), pa_codes<0x4341>(c[0]), pa_codes<0x4240>(c[1]), pa_codes<0x4341>(c[1])};
-                    const uint32_t a1[4] = {pa_codes<0x4240>(c[2]), pa_codes<0x4341>(c[2]), pa_codes<0x4240>(c[3]), pa_codes<0x4341>(c[3])};
-                    few_mma(ot[j], a0, pw);
-                    few_mma(ot[j + 1], a1, pw);
-                }
+                __syncwarp();      // the stage has been read by all lanes
+                if (lane == 0) pa_bar_arrive(empty + 8 * stage);
+                if (++stage == F::STAGES) { stage = 0; ++round; }
             }
-            __syncwarp();      // the stage has been read by all lanes
-            if (lane == 0) pa_bar_arrive(empty + 8 * stage);
-            if (++stage == F::STAGES) { stage = 0; ++round; }
-        }
+        };
+        if (FINE && low) attend(std::integral_constant<bool, FINE>());
+        else attend(std::false_type());
         // the warps' states side by side, merged into the block's
         few_sync();      // the last item's states have been read
 #pragma unroll
@@ -377,17 +394,19 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) pattn_few_kernel(PagesAttn a, 
 
 int pattn_few_status() { return pattn_status_of(g_pattn_status); }
 
-template <int HD>
+template <int HD, bool FINE>
 static void launch_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
-    cudaFuncSetAttribute(pattn_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<HD>::SMEM);
-    launch(pattn_few_kernel<HD>, (unsigned) pattn_blocks(), FEW_THREADS, Few<HD>::SMEM, s, a, tk, tv);
+    cudaFuncSetAttribute(pattn_few_kernel<HD, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<HD>::SMEM);
+    launch(pattn_few_kernel<HD, FINE>, (unsigned) pattn_blocks(), FEW_THREADS, Few<HD>::SMEM, s, a, tk, tv);
     launch_pattn_merge(s, a, pattn_blocks());
     count_launch(2);
 }
 
 void launch_pattn_few(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
-    if (a.p.hd == 128) launch_few<128>(s, a, tk, tv);
-    else launch_few<64>(s, a, tk, tv);
+    const bool fine = a.q_type == NSL_F32;
+    if (a.p.hd == 128) { if (fine) launch_few<128, true>(s, a, tk, tv); else launch_few<128, false>(s, a, tk, tv); }
+    else if (fine) launch_few<64, true>(s, a, tk, tv);
+    else launch_few<64, false>(s, a, tk, tv);
 }
 
 }   // namespace nsl

@@ -9,6 +9,8 @@
 // codes to f16 (exact) into the layout the products read, 1 fetches pages, 1 issues the scores' products (a tile's next unit as
 // soon as the last scores are in registers), 1 the values' (once the weights are there).  An item of up to 128 columns has both
 // tiles work on the same queries, every other unit each, and their states joined at its end.
+// f32 calls (FINE) add the products of the queries' second f16 terms, from shared memory, where an item has any that are not 0; the room for them is
+// two of the four expanded stages at heads of 128 (4096 rows behind 4096 positions: 319 us as bf16 values in f32 arrays, 352 where the call does not say so, 409 with f32 values).
 // The two scales and the running maxima are as in pages_attn_few.cu; here the maxima that the exponents use follow the true ones
 // only when these have grown by 2^8 (weights up to 2^8 then), so O in tensor memory is hardly ever rescaled.
 // Bound: a unit of two tiles takes 1024 clk of exponentials (16 a clock and SM), 1250 clk of products (the second tile's scores read
@@ -22,26 +24,30 @@
 
 namespace nsl {
 
-constexpr int MANY_KEYS = 64, MANY_TILE = 128, MANY_COLS = PATTN_MANY, MANY_THREADS = 480, MANY_RAW = 3, MANY_STAGES = 4, MANY_META = 16;
+constexpr int MANY_KEYS = 64, MANY_TILE = 128, MANY_COLS = PATTN_MANY, MANY_THREADS = 480, MANY_RAW = 3, MANY_META = 16;
 constexpr int MANY_EXPAND = 8, MANY_FETCH = 12, MANY_SCORES = 13, MANY_VALUES = 14;      // first warp of each part; the softmax has warps 0 .. 7
 constexpr int TM_S = 0, TM_Q = 128, TM_W = 192, TM_O = 256;         // tensor memory columns: S (64 a tile), the first tile's Q (64), W (32 a tile), O (128 a tile)
 constexpr float MANY_SLACK = 8.0f;                                   // how far (in powers of 2) a weight may exceed 1
 
-template <int HD>
+// FINE: queries as two f16 terms (f32 calls).  The second terms of both tiles take the place of two stages at heads of 128.
+template <int HD, bool FINE>
 struct Many {
+    static constexpr int STAGES = FINE && HD == 128 ? 2 : 4;
     static constexpr int RAW = MANY_KEYS * HD;                       // bytes of a unit's key codes, or value codes
     static constexpr int TILE = 2 * RAW;                             // the same as f16
+    static constexpr int QUERIES = 2 * MANY_TILE * HD;               // bytes of a tile's queries as f16
     static constexpr int OFF_TILES = MANY_RAW * 2 * RAW;
-    static constexpr int OFF_Q = OFF_TILES + MANY_STAGES * 2 * TILE; // the second tile's queries
-    static constexpr int OFF_META = OFF_Q + 2 * MANY_TILE * HD;
+    static constexpr int OFF_Q = OFF_TILES + STAGES * 2 * TILE;      // the second tile's queries
+    static constexpr int OFF_QLOW = OFF_Q + QUERIES;                 // FINE: both tiles' second terms
+    static constexpr int OFF_META = OFF_QLOW + (FINE ? 2 * QUERIES : 0);
     static constexpr int OFF_BARS = OFF_META + MANY_META * 4 * 16;
-    static constexpr int BARS = 2 * MANY_RAW + 2 * MANY_STAGES + MANY_META + 11;
+    static constexpr int BARS = 2 * MANY_RAW + 2 * STAGES + MANY_META + 11;
     static constexpr int SMEM = OFF_BARS + 8 * BARS + 1024;
 };
 static_assert(MANY_COLS == 2 * MANY_TILE, "two tiles an item");
-static_assert(Many<128>::SMEM + 2048 <= 232448, "shared memory");
+static_assert(Many<128, false>::SMEM + 2048 <= 232448 && Many<128, true>::SMEM + 2048 <= 232448, "shared memory");
 constexpr int MANY_SEQS = 4096;      // descriptors of a call; their units sit in the tiles' memory while the plan is made
-static_assert(MANY_SEQS * 4 <= MANY_STAGES * 4 * 64 * 64, "the plan's memory");
+static_assert(MANY_SEQS * 4 <= 4 * 4 * 64 * 64, "the plan's memory: four stages at heads of 64, two or four at 128");
 
 __device__ int g_pattn_many_status;
 
@@ -170,10 +176,12 @@ __device__ __forceinline__ void many_sts(uint32_t at, uint32_t a, uint32_t b, ui
 }
 
 // A column's query divided by its power of two, as f16 to tensor memory (tq) or, tq = 0, to its row of the shared panels of 64 dims
-// (at sq; sx: the row's swizzle).  -> |scale| log2 e times that power.  Out of line, as its registers would be taken from the
+// (at sq; sx: the row's swizzle); FINE: what that rounding left off, as f16 again, to panels at sl.  -> |scale| log2 e times that
+// power, and whether anything was left off.  Out of line, as its registers would be taken from the
 // softmax, and in short loops: code that runs once an item is fetched anew each time, and unrolled it took 10 us an item.
-template <int HD>
-static __device__ __noinline__ float many_query(const PagesAttn& a, size_t at, bool valid, uint32_t tq, uint32_t sq, uint32_t sx) {
+struct ManyQuery { float f; bool low; };
+template <int HD, bool FINE>
+static __device__ __noinline__ ManyQuery many_query(const PagesAttn& a, size_t at, bool valid, uint32_t tq, uint32_t sq, uint32_t sl, uint32_t sx) {
     const bool packed = a.q_type == NSL_BF16;
     float top = 0.0f;
     if (valid) {
@@ -198,6 +206,7 @@ static __device__ __noinline__ float many_query(const PagesAttn& a, size_t at, b
         }
     }
     const float by = pa_pow2_of(top), inv = copysignf(1.0f / by, a.scale);      // the scale's sign goes with the query: maxima are then of scores
+    uint32_t low = 0;
 #pragma unroll 1
     for (int d = 0; d < HD; d += 32) {
         uint32_t w[16];
@@ -220,10 +229,19 @@ static __device__ __noinline__ float many_query(const PagesAttn& a, size_t at, b
 #pragma unroll
             for (int j = 0; j < 4; ++j) many_sts(sq + (d >> 6) * (MANY_TILE * 128) + (((uint32_t) ((d & 63) / 8 + j) ^ sx) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
         }
+        if (FINE) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { w[e] = pa_low_f16x2(v[2 * e] * inv, v[2 * e + 1] * inv, w[e]); low |= w[e]; }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) many_sts(sl + (d >> 6) * (MANY_TILE * 128) + (((uint32_t) ((d & 63) / 8 + j) ^ sx) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        }
     }
     if (tq) tm_wait_st();
-    else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    return fabsf(a.scale) * 1.4426950408889634f * by;
+    if (FINE || !tq) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    ManyQuery r;
+    r.f = fabsf(a.scale) * 1.4426950408889634f * by;
+    r.low = (low & 0x7FFF7FFFu) != 0;
+    return r;
 }
 
 // A column's O (and, second: the other tile's, 128 columns on) out of tensor memory, times by and by1: to a state (part: columns side by
@@ -254,26 +272,27 @@ static __device__ __noinline__ void many_results(const PagesAttn& a, uint32_t to
 }
 
 // WIDE: pages of 64 and more positions, a unit's keys have one pair of scales.
-template <int HD, bool WIDE>
+template <int HD, bool WIDE, bool FINE>
 __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __grid_constant__ PagesAttn a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
-    using F = Many<HD>;
-    constexpr int STATE = PATTN_STATE<HD>, WARPS = MANY_THREADS / 32, NG = WIDE ? 1 : 4, GK = MANY_KEYS / NG;      // groups of GK keys with one pair of scales
+    using F = Many<HD, FINE>;
+    constexpr int STAGES = F::STAGES, STATE = PATTN_STATE<HD>, WARPS = MANY_THREADS / 32, NG = WIDE ? 1 : 4, GK = MANY_KEYS / NG;      // groups of GK keys with one pair of scales
     extern __shared__ uint8_t many_raw[];
     uint8_t* const smem = (uint8_t*) (((uintptr_t) many_raw + 1023) & ~(uintptr_t) 1023);
     __shared__ int wsum[WARPS], plan[2], abort_flag;
     __shared__ uint32_t tmem_slot;
+    __shared__ int q_low[MANY_EXPAND];      // FINE, by softmax warp: do its columns' queries have second terms that are not 0
     __shared__ float other[3][MANY_TILE];      // the second tile's m, l, mo where both have the same columns
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.n_head / a.p.n_kv;
     const uint32_t base = pa_smem(smem), tiles = base + F::OFF_TILES, bars = base + F::OFF_BARS;
     // arrivals: raw_full the fetch (and bytes), raw_empty the 4 expanding warps, tile_full the same, tile_empty the products, meta the fetch;
     // per tile: s_full and o_done (a unit's scores are there, its values are in O) the products, s_free (the scores are in registers),
     // w_full and q_full the tile's 4 warps; done the warps that issue products
-    const uint32_t raw_full = bars, raw_empty = raw_full + 8 * MANY_RAW, tile_full = raw_empty + 8 * MANY_RAW, tile_empty = tile_full + 8 * MANY_STAGES, meta_full = tile_empty + 8 * MANY_STAGES,
+    const uint32_t raw_full = bars, raw_empty = raw_full + 8 * MANY_RAW, tile_full = raw_empty + 8 * MANY_RAW, tile_empty = tile_full + 8 * STAGES, meta_full = tile_empty + 8 * STAGES,
                    s_full = meta_full + 8 * MANY_META, s_free = s_full + 16, w_full = s_free + 16, q_full = w_full + 16, o_done = q_full + 16, done = o_done + 16;
     const float4* const meta = (const float4*) (smem + F::OFF_META);
     if (tid == 0) {
         for (int i = 0; i < MANY_RAW; ++i) { pa_bar_init(raw_full + 8 * i, 1); pa_bar_init(raw_empty + 8 * i, 4); }
-        for (int i = 0; i < MANY_STAGES; ++i) { pa_bar_init(tile_full + 8 * i, 4); pa_bar_init(tile_empty + 8 * i, 1); }
+        for (int i = 0; i < STAGES; ++i) { pa_bar_init(tile_full + 8 * i, 4); pa_bar_init(tile_empty + 8 * i, 1); }
         for (int i = 0; i < MANY_META; ++i) pa_bar_init(meta_full + 8 * i, 1);
         for (int t = 0; t < 2; ++t) { pa_bar_init(s_full + 8 * t, 1); pa_bar_init(s_free + 8 * t, 4); pa_bar_init(w_full + 8 * t, 4); pa_bar_init(q_full + 8 * t, 4); pa_bar_init(o_done + 8 * t, 1); }
         pa_bar_init(done, 2);
@@ -342,8 +361,15 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
             const int row = it.sp.row + col / group, head = it.kvh * group + col % group, pos = pos_of(it.sp.pos, col / group);
             const int hi = valid ? pos : -1, lo = valid ? first_key(a, pos) : 0;
             float f = 0.0f;      // scale, log2 e and the power of two that the query is divided by
+            bool low = false;
             if (warp_valid) {
-                f = many_query<HD>(a, (size_t) row * a.q_stride + (size_t) head * HD, valid, t == 0 ? lanes + TM_Q : 0u, base + F::OFF_Q + c * 128, c & 7);
+                const ManyQuery mq = many_query<HD, FINE>(a, (size_t) row * a.q_stride + (size_t) head * HD, valid, t == 0 ? lanes + TM_Q : 0u, base + F::OFF_Q + c * 128, base + F::OFF_QLOW + t * F::QUERIES + c * 128, c & 7);
+                f = mq.f;
+                low = FINE && mq.low;
+            }
+            if (FINE) {
+                low = __any_sync(0xFFFFFFFFu, low);
+                if (lane == 0) q_low[warp] = low;
             }
             tm_before();
             __syncwarp();
@@ -513,9 +539,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
         const int odd = lane >> 4, half = lane >> 3 & 1;
         const uint32_t v_to = (uint32_t) F::TILE + (uint32_t) (8 * odd + (lane & 7)) * 128 + (((uint32_t) (2 * w + half) ^ (uint32_t) (lane & 7)) << 4);
         for (int n = xe - x0; g < n; ++g) {
-            const uint32_t rs = (uint32_t) (g % MANY_RAW), st = (uint32_t) (g % MANY_STAGES);
+            const uint32_t rs = (uint32_t) (g % MANY_RAW), st = (uint32_t) (g % STAGES);
             wait(raw_full + 8 * rs, g / MANY_RAW & 1, 7);
-            if (g >= MANY_STAGES) wait(tile_empty + 8 * st, (g / MANY_STAGES - 1) & 1, 8);
+            if (g >= STAGES) wait(tile_empty + 8 * st, (g / STAGES - 1) & 1, 8);
             const uint32_t raw = base + rs * 2 * F::RAW, out = tiles + st * 2 * F::TILE;
             // keys: row and chunk of 16 codes a thread -> two 16-byte pieces of the row's f16 values
 #pragma unroll
@@ -598,21 +624,27 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
         // everything that an operand is made of comes from constants, counters and values that the warp is known to share (same())
         constexpr uint32_t id_s = many_idesc(MANY_KEYS), id_o = many_idesc(HD);
         const bool scores = warp == MANY_SCORES;
-        const uint64_t qd = many_desc(base + F::OFF_Q), kd0 = many_desc(tiles), vd0 = many_desc(tiles + F::TILE);
+        const uint64_t qd = many_desc(base + F::OFF_Q), qlow = many_desc(base + F::OFF_QLOW), kd0 = many_desc(tiles), vd0 = many_desc(tiles + F::TILE);
         uint32_t items = 0, units = 0, issued[2] = {0, 0};      // of this block so far; of a tile: units
         for (int x = x0; walk.next(a, group, x, xe, &it); x = it.x1, ++items) {
             const uint32_t run = same(it.x1 - it.x0), shared = same(it.cols <= MANY_TILE), n = shared ? run : 2 * run;
+            uint32_t low[2] = {0, 0};      // of a tile: its queries have second terms
             if (scores) {
                 wait(q_full, items & 1, 10);
                 wait(q_full + 8, items & 1, 10);
                 tm_after();
+                if (FINE) {
+                    const uint32_t mine = lane < MANY_EXPAND ? (uint32_t) ((volatile int*) q_low)[lane] << lane : 0u, all = same(mine);
+                    low[0] = all & 0xFu;
+                    low[1] = all >> 4;
+                }
             }
             auto step = [&](auto tile, uint32_t i) {      // of tile i & 1
                 constexpr int t = decltype(tile)::value;
                 if (i >= n) return;
-                const uint32_t at = units + (shared ? i : i >> 1), stage = at % MANY_STAGES;
+                const uint32_t at = units + (shared ? i : i >> 1), stage = at % STAGES;
                 if (scores) {
-                    wait(tile_full + 8 * stage, at / MANY_STAGES & 1, 11);
+                    wait(tile_full + 8 * stage, at / STAGES & 1, 11);
                     if (issued[t] > 0) wait(s_free + 8 * t, (issued[t] - 1) & 1, 12);
                     tm_after();
                     const uint64_t kd = kd0 + (uint64_t) (stage * (2 * F::TILE >> 4));
@@ -622,6 +654,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
                         if (t == 0) many_mma(TM_S, TM_Q + 8 * k, kk, id_s, k > 0);
                         else many_mma_smem(TM_S + 64, qd + (uint64_t) (((k >> 2) * (MANY_TILE * 128) + (k & 3) * 32) >> 4), kk, id_s, k > 0);
                     }
+                    if (FINE && low[t])
+#pragma unroll
+                        for (int k = 0; k < HD / 16; ++k) {
+                            const uint64_t at_k = (uint64_t) ((t * F::QUERIES + (k >> 2) * (MANY_TILE * 128) + (k & 3) * 32) >> 4);
+                            many_mma_smem(TM_S + 64 * t, qlow + at_k, kd + (uint64_t) (((k >> 2) * (MANY_KEYS * 128) + (k & 3) * 32) >> 4), id_s, true);
+                        }
                     many_commit(s_full + 8 * t);
                 } else {
                     wait(w_full + 8 * t, issued[t] & 1, 13);
@@ -716,14 +754,20 @@ __global__ void __launch_bounds__(JOIN_THREADS) pattn_join_kernel(const __grid_c
     }
 }
 
-template <int HD, bool WIDE>
+template <int HD, bool WIDE, bool FINE>
 static void launch_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
     const unsigned blocks = (unsigned) sm_count();
-    cudaFuncSetAttribute(pattn_many_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<HD>::SMEM);
-    launch(pattn_many_kernel<HD, WIDE>, blocks, MANY_THREADS, Many<HD>::SMEM, s, a, tk, tv);
+    constexpr int SMEM = Many<HD, FINE>::SMEM;
+    cudaFuncSetAttribute(pattn_many_kernel<HD, WIDE, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    launch(pattn_many_kernel<HD, WIDE, FINE>, blocks, MANY_THREADS, SMEM, s, a, tk, tv);
     const int cols = (a.n_head / a.p.n_kv) * a.max_rows;
     launch(pattn_join_kernel<HD>, dim3(blocks, (unsigned) (cols < MANY_COLS ? (cols + JOIN_COLS - 1) / JOIN_COLS : MANY_COLS / JOIN_COLS)), JOIN_THREADS, 0, s, a);
     count_launch(2);
+}
+template <int HD, bool WIDE>
+static void launch_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {
+    if (a.q_type == NSL_F32) launch_many<HD, WIDE, true>(s, a, tk, tv);
+    else launch_many<HD, WIDE, false>(s, a, tk, tv);
 }
 
 void launch_pattn_many(cudaStream_t s, const PagesAttn& a, const CUtensorMap& tk, const CUtensorMap& tv) {

@@ -194,9 +194,10 @@ class PagePool:
         self.lib.nsl_pages_read(_stream(self.index), self._p, layer, _type(k_out, rounded), _ptr(k_out), ks, _ptr(v_out), vs, _ptr(rows), n, shape[0])
         _done()
 
-    def attn(self, layer, q, rows, out, max_rows, scale=None, window=0, work=None):
+    def attn(self, layer, q, rows, out, max_rows, scale=None, window=0, work=None, rounded=False):
         """Causal attention of q [T][heads][hd] over the sequences' pages -> out (bfloat16, or float32 rounded to bf16).  Each stream and each
-        captured graph has work memory of its own (40 MB); work: another one (int32).  NaN in a row whose query is finite: a wait on the
+        captured graph has work memory of its own (40 MB); work: another one (int32).  float32 queries take part with 22 bits; rounded: they hold bf16
+        values (what rope and append give with rounded=True), and 11 bits do.  NaN in a row whose query is finite: a wait on the
         device ran out, see status()."""
         _here(self.index, q, rows, out, work)
         qs, os, (T, heads, hd) = _rows(q, "q"), _rows(out, "out"), q.shape
@@ -208,7 +209,7 @@ class PagePool:
         stream = _stream(self.index)
         if work is None:
             work = self._work_of(stream)
-        self.lib.nsl_pages_attn(stream, self._p, layer, _type(q), _ptr(q), qs, heads, hd ** -0.5 if scale is None else scale, window, _ptr(rows), n, max_rows, T,
+        self.lib.nsl_pages_attn(stream, self._p, layer, _type(q, rounded), _ptr(q), qs, heads, hd ** -0.5 if scale is None else scale, window, _ptr(rows), n, max_rows, T,
                                 _type(out, True), _ptr(out), os, _ptr(work))
         _done()
 

@@ -386,3 +386,51 @@ def test_attn_of_single_rows_beyond_32_bits(hd, page):
     pool = P().PagePool(k, v, ks, vs, torch.ones(pages, dtype=torch.int32, device="cuda"), ints([ids, ids[::-1]]), ints([5 * page] * 2))
     q = torch.randn(2, 16, hd, generator=g, device="cuda").to(torch.bfloat16)
     check_attn(pool, q, [[0, 1, 5 * page - 1, 0], [1, 1, 3 * page + 2, 1]], layer=0)
+
+
+# ---- queries with all of float32's bits ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,group,hd,page", [(1, 8, 128, 64), (1, 4, 64, 16), (2, 4, 64, 128), (1, 1, 128, 16), (6, 8, 64, 32), (3, 16, 128, 64), (70, 8, 128, 16), (200, 4, 128, 128), (150, 2, 64, 64)], ids=str)
+@pytest.mark.parametrize("size", [1.0, 8.0, 32.0])
+def test_attn_float32_queries(rows, group, hd, page, size):
+    """Queries with 24 significant bits: the tolerance has no term for them.  Scores are as large as the queries make them, so their f32 sums' share grows with
+    size: hd products, each rounded once more in the sum (2^-24 of sum |q k| scale each), and 2^-24 of the largest query by the keys' sum for the queries themselves."""
+    g = gen_of(rows + page + int(size))
+    n = 1500
+    pool = random_pool(g, 2, -(-n // page) + 2, 2, hd, page, [n])
+    pool.ks.fill_(2.0 ** -6)
+    pool.k.copy_((torch.randn(pool.k.shape, generator=g, device="cuda") * 36).round().clamp(-127, 127).to(torch.int8))
+    q = torch.randn(rows, 2 * group, hd, generator=g, device="cuda") * size
+    seqs = [[0, rows, n - rows, 0]]
+    o = torch.full(q.shape, 5.0, device="cuda")
+    pool.attn(1, q, ints(seqs), o, max_rows=rows)
+    want, total = attn64(pool, 1, q, seqs, hd ** -0.5, 0)
+    scale = hd ** -0.5
+    k = held(pool, 1, 0, n)[0]      # [n][kv][hd]
+    s = torch.einsum("ngd,rgjd->rgjn", k.abs(), q.double().abs().view(rows, 2, group, hd)).amax(-1) * scale      # the largest sum |q k| scale of a column
+    top = (q.double().abs().amax(-1).view(rows, 2, group) * k.abs().sum(-1).amax(0)[None, :, None]) * scale
+    off = 2 * (hd * F32 * s + 2 * F32 * top + 4 * F32 * s)      # of a weight, relative: in numerator and sum
+    # a weight times its page's value scale is held as f16: 2^-11 of it, or, below 2^-14 of the largest such product, half a subnormal step, 2^-25 of the
+    # largest, by the code that it multiplies.  That is next to nothing of the row, but can be all of an element to which the heaviest keys add codes of 0.
+    p64 = torch.einsum("ngd,rgjd->rgjn", k, q.double().view(rows, 2, group, hd)) * scale
+    p64 = p64.masked_fill(torch.arange(n, device="cuda") > torch.arange(n - rows, n, device="cuda")[:, None, None, None], -math.inf).softmax(-1)
+    at = torch.arange(n, device="cuda")
+    vs = pool.vs[1, pool.table[0, at // page].long()].double()      # [n][kv]
+    most = (p64 * vs.T[None, :, None]).amax(-1)      # [rows][kv][group]
+    codes = (held(pool, 1, 0, n)[1] / vs[..., None]).abs().sum(0)      # [kv][hd]
+    small = 2.0 ** -25 * (most[..., None] * codes[None, :, None]).reshape(rows, 2 * group, hd)
+    tol = ((2.0 ** -11 + off.view(rows, 2 * group, 1)) * total + small) * (1 + BF16) + BF16 * want.abs()
+    far = ((o.double() - want).abs() / tol).max()
+    assert float(far) <= 1.0
+
+
+@pytest.mark.parametrize("rows,group,hd,page", [(1, 8, 128, 64), (6, 8, 64, 32), (200, 4, 128, 16)], ids=str)
+def test_attn_float32_arrays_of_bf16_values(rows, group, hd, page):
+    """The same bits as bf16 queries, said to be rounded or not."""
+    g = gen_of(61)
+    pool = random_pool(g, 2, -(-900 // page) + 2, 2, hd, page, [900])
+    q = torch.randn(rows, 2 * group, hd, generator=g, device="cuda").to(torch.bfloat16)
+    rows_, outs = ints([[0, rows, 900 - rows, 0]]), []
+    for x, more in ((q, {}), (q.float(), {}), (q.float(), {"rounded": True})):
+        outs.append(torch.empty_like(q))
+        pool.attn(1, x, rows_, outs[-1], max_rows=rows, **more)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
