@@ -39,8 +39,12 @@ typedef struct {
  *   NSL_ROPE_PLAIN   theta^(-2 p / rot)
  *   NSL_ROPE_LINEAR  the same / scale (positions interpolated)
  *   NSL_ROPE_BASE    theta * scale^(rot / (rot - 2)) instead of theta: the lowest frequency is divided by scale, the highest kept
- *   NSL_ROPE_PARTS   frequencies that turn more than beta_fast times within ctx positions are kept, those below beta_slow
- *                    turns divided by scale, a linear ramp over p between (YaRN, arXiv 2309.00071, eq. 17-23); factor = 0.1 ln(scale) + 1
+ *   NSL_ROPE_PARTS  frequencies that turn more than beta_fast times within ctx positions are kept, those below beta_slow turns divided
+ *                    by scale, and between them r of the way: with c(beta) = rot ln(ctx / (2 pi beta)) / (2 ln theta), the pair that turns beta
+ *                    times, lo = max(floor c(beta_fast), 0), hi = min(ceil c(beta_slow), rot - 1), at least lo + 0.001, and
+ *                    r = (p - lo) / (hi - lo) within [0, 1], times (1 - r) + r / scale; factor = 0.1 ln(scale) + 1.  The idea is YaRN's (arXiv
+ *                    2309.00071); its eq. 17-23 have a ramp that is linear in the turns, while this one, linear in the pair's number, is the one
+ *                    that models with such tables are published for (pair 33 of rot 128, theta 1e4, ctx 4096, scale 16: 4.60e-3, by the turns 1.76e-3)
  * -> 0, or -1 with a message (rot not even and positive, theta <= 1, scale < 1, or ctx / betas unusable). */
 enum { NSL_ROPE_PLAIN = 0, NSL_ROPE_LINEAR = 1, NSL_ROPE_BASE = 2, NSL_ROPE_PARTS = 3 };
 int nsl_rope_freqs(int kind, int rot, double theta, double scale, int ctx, double beta_fast, double beta_slow, float* inv, float* factor);

@@ -54,7 +54,7 @@ int nsl_rope_freqs(int kind, int rot, double theta, double scale, int ctx, doubl
     }
     const int n = rot / 2;
     const double base = kind == NSL_ROPE_BASE ? theta * pow(scale, rot / (rot - 2.0)) : theta;
-    // the pair (as a real number) whose frequency turns `beta` times within ctx positions
+    // the pair (as a real number) whose frequency turns `beta` times within ctx positions; the ramp between two of them is linear in the pair's number
     auto pair_of = [&](double beta) { return rot * log(ctx / (beta * 6.283185307179586)) / (2.0 * log(theta)); };
     double lo = 0.0, hi = 0.0;
     if (kind == NSL_ROPE_PARTS) {

@@ -75,3 +75,16 @@ def test_a_call_reports_nothing_of_other_threads():
     t.join()
     assert seen[0].startswith(b"nsl_pages_fork") and lib.nsl_pages_error() == b""
     lib.nsl_last_error()
+
+
+# ---- frequencies by parts: known values, worked out apart from the code (40 decimal digits), to half a step of float32 (2^-24) -----------
+@pytest.mark.parametrize("rot,scale,factor,values", [
+    (128, 16.0, 1.277258872223978, {0: 1.0, 10: 2.371373705661655e-1, 20: 5.623413251903491e-2, 21: 4.694085999795940e-2, 33: 4.600435467850347e-3, 45: 1.517716047318249e-4,
+                                    46: 8.334508951020775e-5, 63: 7.217387404309114e-6}),      # pairs 20.94 and 45.03: the ramp from 20 to 46
+    (64, 40.0, 1.368887945411394, {0: 1.0, 10: 5.623413251903491e-2, 11: 3.900692656714386e-2, 16: 5.5e-3, 22: 1.778279410038923e-4, 23: 3.333803580408310e-5,
+                                   31: 3.333803580408310e-6})])                                # pairs 10.47 and 22.51: from 10 to 23
+def test_known_frequencies_by_parts(rot, scale, factor, values):
+    inv, f = P.rope_freqs(rot, 1e4, P.ROPE_PARTS, scale, 4096)
+    assert abs(f - factor) <= 2.0 ** -24 * factor * 1.001
+    for p, want in values.items():
+        assert abs(float(inv[p]) - want) <= 2.0 ** -24 * want * 1.001, p
