@@ -45,7 +45,7 @@ typedef struct {
  *                    r = (p - lo) / (hi - lo) within [0, 1], times (1 - r) + r / scale; factor = 0.1 ln(scale) + 1.  The idea is YaRN's (arXiv
  *                    2309.00071); its eq. 17-23 have a ramp that is linear in the turns, while this one, linear in the pair's number, is the one
  *                    that models with such tables are published for (pair 33 of rot 128, theta 1e4, ctx 4096, scale 16: 4.60e-3, by the turns 1.76e-3)
- * -> 0, or -1 with a message (rot not even and positive, theta <= 1, scale < 1, or ctx / betas unusable). */
+ * -> 0, or -1 with a message (rot not even and positive, theta <= 1 or scale < 1 or not finite, or ctx / betas unusable). */
 enum { NSL_ROPE_PLAIN = 0, NSL_ROPE_LINEAR = 1, NSL_ROPE_BASE = 2, NSL_ROPE_PARTS = 3 };
 int nsl_rope_freqs(int kind, int rot, double theta, double scale, int ctx, double beta_fast, double beta_slow, float* inv, float* factor);
 /* Rows of heads rotated: x = factor (u cos a - w sin a, w cos a + u sin a), a = pos[t] * inv[p], the product reduced to a

@@ -47,7 +47,7 @@ extern "C" {
 
 int nsl_rope_freqs(int kind, int rot, double theta, double scale, int ctx, double beta_fast, double beta_slow, float* inv, float* factor) {
     begin_call();
-    if (kind < NSL_ROPE_PLAIN || kind > NSL_ROPE_PARTS || rot < 2 || rot % 2 || !(theta > 1.0) || !(scale >= 1.0) || !inv || !factor || (kind == NSL_ROPE_BASE && rot < 4) ||
+    if (kind < NSL_ROPE_PLAIN || kind > NSL_ROPE_PARTS || rot < 2 || rot % 2 || !(theta > 1.0) || !(scale >= 1.0) || !isfinite(theta) || !isfinite(scale) || !inv || !factor || (kind == NSL_ROPE_BASE && rot < 4) ||
         (kind == NSL_ROPE_PARTS && (ctx < 1 || !(beta_fast > beta_slow) || !(beta_slow > 0.0)))) {
         set_error("nsl_rope_freqs: kind %d, %d rotated values, theta %g, scale %g, %d positions, betas %g and %g", kind, rot, theta, scale, ctx, beta_fast, beta_slow);
         return -1;

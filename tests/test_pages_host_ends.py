@@ -88,3 +88,9 @@ def test_known_frequencies_by_parts(rot, scale, factor, values):
     assert abs(f - factor) <= 2.0 ** -24 * factor * 1.001
     for p, want in values.items():
         assert abs(float(inv[p]) - want) <= 2.0 ** -24 * want * 1.001, p
+
+
+@pytest.mark.parametrize("args", [(64, float("inf")), (64, 1e4, P.ROPE_LINEAR, float("inf")), (64, 1e4, P.ROPE_BASE, float("inf")), (64, 1e4, P.ROPE_PARTS, float("inf"), 4096)], ids=str)
+def test_frequencies_of_infinite_arguments(args):
+    with pytest.raises(ValueError, match="nsl_rope_freqs"):
+        P.rope_freqs(*args)
