@@ -434,3 +434,129 @@ def test_attn_float32_arrays_of_bf16_values(rows, group, hd, page):
         outs.append(torch.empty_like(q))
         pool.attn(1, x, rows_, outs[-1], max_rows=rows, **more)
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+# ---- calls that the documentation allows and the other tests do not make -----------------------------------------------------------------------
+@pytest.mark.parametrize("heads,kv,rows", [(300, 1, 1), (272, 1, 3), (1040, 2, 1), (600, 2, 2)])
+def test_attn_of_more_heads_than_an_item_has_columns(heads, kv, rows):
+    g = gen_of(heads)
+    pool = random_pool(g, 2, 30, kv, 64, 32, [500, 90])
+    q = torch.randn(2 * rows, heads, 64, generator=g, device="cuda").to(torch.bfloat16)
+    check_attn(pool, q, [[0, rows, 500 - rows, 0], [rows, rows, 90 - rows, 1]])
+    check_attn(pool, q, [[0, rows, 500 - rows, 0], [rows, rows, 90 - rows, 1]], window=70)
+
+
+@pytest.mark.parametrize("n,heads", [(1000, 16), (4096, 16), (4096, 4)])
+def test_attn_padded_batches_of_many_sequences(n, heads):
+    """Every third place of the batch is empty, in either attention kernel; the list is as long as it may be."""
+    g = gen_of(n)
+    lens = [1 + (53 * i) % 200 for i in range(n)]
+    pool = random_pool(g, 2, sum(-(-m // 32) for m in lens), 1, 64, 32, lens)
+    q = torch.randn(n, heads, 64, generator=g, device="cuda").to(torch.bfloat16)
+    check_attn(pool, q, [[i, 0 if i % 3 == 1 else 1, m - 1, i] for i, m in enumerate(lens)])
+
+
+def test_append_of_many_rows_with_heads_that_do_not_divide():
+    """Blocks with several rows of queries and several of the three KV heads; read back with several rows a block."""
+    g = gen_of(62)
+    kv, hd, page, seqs = 3, 64, 16, [(5, 9000), (0, 1), (31, 500), (16, 16)]
+    lengths = [p + n for p, n in seqs]
+    pool = random_pool(g, 2, sum(-(-m // page) for m in lengths) + 3, kv, hd, page, lengths)
+    T = sum(n for _, n in seqs)
+    q, k, v = (torch.randn(T, h, hd, generator=g, device="cuda").to(torch.bfloat16) for h in (5, kv, kv))
+    desc, row = [], 0
+    for s, (p, n) in enumerate(seqs):
+        desc += [[row, n, p, s], [T, 5, 3, 1]]      # and places behind the call's rows
+        row += n
+    before = [(a.clone(), b.clone()) for a, b in ((pool.k, pool.ks), (pool.v, pool.vs))]
+    r, qo = P().Rope(inv_of(32)), torch.empty_like(q)
+    pool.append(1, r, q, k, v, ints(desc), qo)
+    pos = torch.cat([torch.arange(p, p + n, device="cuda") for p, n in seqs])
+    for x, got in ((q, qo),):
+        want, size = turned(x, pos, r.inv, False, 1.0)
+        assert bool(((got.double() - want).abs() <= BF16 * want.abs() + (1 + BF16) * 4 * F32 * size).all())
+    kr, size = turned(k, pos, r.inv, False, 1.0)
+    kb, vb = torch.empty_like(k), torch.empty_like(v)
+    pool.read(1, ints(desc), kb, vb)
+    for codes, scales, was, x, tol, back in ((pool.k, pool.ks, before[0], kr, 4 * F32 * size, kb), (pool.v, pool.vs, before[1], v.double(), 0 * size, vb)):
+        row = 0
+        for s, (p, n) in enumerate(seqs):
+            ids, at = pool.table[s].long(), torch.arange(p, p + n, device="cuda")
+            pid = ids[at // page]
+            scale = scales[1, pid].double()      # [n][kv]
+            mine = x[row:row + n]
+            # of each page: the power of two for its new rows, or the old scale where rows were there before and theirs was larger
+            top = torch.zeros(codes.shape[1], kv, dtype=torch.float64, device="cuda").scatter_reduce(0, pid[:, None].expand(-1, kv), mine.abs().amax(-1), "amax")
+            m, e = torch.frexp(top)      # top = m 2^e, m in [1/2, 1): top <= 127 2^(e - 7) where m <= 127 / 128
+            need = torch.ldexp(torch.ones_like(top), torch.where(m <= 127 / 128, e - 7, e - 6))
+            first = int(ids[p // page])
+            if p % page:
+                need[first] = torch.maximum(need[first], was[1][1, first].double())
+            assert torch.equal(scale, need[pid])
+            held_now = codes[1, pid, :, at % page].double() * scale[..., None]
+            assert bool(((held_now - mine).abs() <= scale[..., None] / 2 + tol[row:row + n]).all())
+            assert torch.equal(back[row:row + n], held_now.float().to(torch.bfloat16))
+            row += n
+
+
+def test_a_captured_step_is_replayed_with_other_lengths():
+    """Management, store and attention captured into one graph, and replayed with descriptors and requests that are changed on the device, against the same
+    calls one by one on another pool."""
+    g = gen_of(63)
+    def build():
+        pool = P().PagePool.empty(2, 60, 2, 64, 16, 4, 12)
+        for t in (pool.k, pool.v, pool.ks, pool.vs):
+            t.zero_()
+        return pool
+    a, b = build(), build()
+    x = torch.randn(12, 3, 4, 8, 64, generator=g, device="cuda").to(torch.bfloat16)
+    r = P().Rope(inv_of(64))
+    ins = [x[0, i].clone() for i in range(3)]
+    rows, grow, forks, cut = ints([[0, 1, 0, 0], [1, 3, 0, 1], [0, 0, 0, 2], [0, 0, 0, 3]]), ints([[0, 1], [1, 3]]), ints([[0, 2, 0, 0]]), ints([[3, 0]])
+    qa, oa = torch.zeros(4, 8, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(4, 8, 64, dtype=torch.bfloat16, device="cuda")
+
+    def step(pool, q2, o):
+        pool.trim(cut)
+        pool.fork(forks)
+        pool.extend(grow)
+        for layer in (0, 1):
+            pool.append(layer, r, ins[0], ins[1][:, :2], ins[2][:, :2], rows, q2)
+            pool.attn(layer, q2, rows, o, max_rows=3)
+        pool.compact()
+
+    graph = torch.cuda.CUDAGraph()
+    state = [t.clone() for t in (a.table, a.ref, a.length)]
+    with torch.cuda.graph(graph):
+        step(a, qa, oa)
+    for t, was in zip((a.table, a.ref, a.length), state):
+        assert torch.equal(t, was)      # capturing runs nothing
+    length = {0: 0, 1: 0}
+    for i in range(12):
+        for j in range(3):
+            ins[j].copy_(x[i, j])
+        plan = [[0, 1, length[0], 0], [1, 3, length[1], 1], [0, 0, 0, 2], [0, 0, 0, 3]]
+        rows.copy_(ints(plan))
+        length[0], length[1] = length[0] + 1, length[1] + 3
+        grow.copy_(ints([[0, length[0]], [1, length[1]]]))
+        forks.copy_(ints([[1, 2, 9, 0] if i == 5 else [0, 0, 0, 0]]))
+        cut.copy_(ints([[2, 0] if i == 9 else [1, length[1]]]))
+        graph.replay()
+        qb, ob = torch.zeros_like(qa), torch.zeros_like(oa)
+        step(b, qb, ob)
+        assert torch.equal(oa, ob) and torch.equal(qa, qb)
+        for s, t in ((a.table, b.table), (a.ref, b.ref), (a.length, b.length)):
+            assert torch.equal(s, t)
+        want, size = attn64(a, 1, qa, plan, 0.125, 0)
+        assert bool(((oa.double() - want).abs() <= BF16 * want.abs() + (1 + BF16) * WEIGHTS * size).all())
+
+
+@pytest.mark.parametrize("offset", [0, 1, 37])
+def test_lists_anywhere_in_memory(offset):
+    """Descriptors and requests of odd offsets in a longer list: 4-byte alignment is all they have."""
+    g = gen_of(64)
+    pool = random_pool(g, 2, 20, 2, 64, 16, [100, 60])
+    q = torch.randn(6, 8, 64, generator=g, device="cuda").to(torch.bfloat16)
+    seqs = [[0, 1, 99, 0], [1, 5, 40, 1]]
+    flat = torch.zeros(offset + 8, dtype=torch.int32, device="cuda")
+    flat[offset:] = ints(seqs).flatten()
+    check_attn(pool, q, seqs, rows=flat[offset:].view(2, 4))
