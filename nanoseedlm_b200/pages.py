@@ -67,10 +67,13 @@ def _ints(t, name, width):
     return shape[0]
 
 
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _here(index, *tensors):
     """All on the device `index`, and that the current one."""
-    if index != torch.cuda.current_device():
-        raise ValueError(f"tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
+    if index < 0 or index != _device():
+        raise ValueError(f"tensors on {f'cuda:{index}' if index >= 0 else 'the host'}, but the current device is cuda:{torch.cuda.current_device()}")
     for t in tensors:
         if t is not None and t.get_device() != index:
             raise ValueError(f"a tensor on {t.device} among tensors on cuda:{index}")
@@ -146,7 +149,7 @@ class PagePool:
 
     def _work_of(self, stream):
         """Attention's work memory: the stream's own, made at its first call; in a capture the graph's, from the capture's memory."""
-        if _capturing():
+        if stream and _capturing():      # (the default stream, 0, is never captured)
             return torch.empty_like(self.attn_work)
         work = self._works.get(stream)
         if work is None:

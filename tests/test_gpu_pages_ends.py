@@ -249,6 +249,16 @@ def test_attn_in_two_graphs_replayed_beside_one_another():
             assert torch.equal(out, alone)
 
 
+def test_host_tensors_are_refused():
+    x, rows = torch.zeros(2, 2, 64), torch.zeros(1, 4, dtype=torch.int32)
+    pool = P().PagePool.empty(1, 4, 2, 64, 16, 2, 2)
+    y = x.cuda()
+    for call in (lambda: P().rope(P().Rope(inv_of(64)), x, None, rows[0, :2]), lambda: P().rope(P().Rope(inv_of(64)), y, None, rows[0, :2]), lambda: pool.attn(0, x, rows.cuda(), x.clone(), max_rows=1),
+                 lambda: pool.attn(0, y, rows.cuda(), torch.empty_like(y), max_rows=1, work=torch.zeros(1 << 24, dtype=torch.int32)), lambda: pool.trim(rows[:, :2].contiguous())):
+        with pytest.raises(ValueError, match="the host|on cpu"):
+            call()
+
+
 # ---- outputs beside inputs ---------------------------------------------------------------------------------------------------------------
 def test_outputs_in_place_and_beside_the_inputs():
     """Rows side by side in wider rows, behind one another, and in place are served; what overlaps is refused and nothing is written."""
