@@ -157,9 +157,12 @@ void nsl_pages_attn(cudaStream_t s, const NslPages* p, int layer, int q_type, co
     a.n_head = n_head; a.layer = layer; a.window = window; a.n_seqs = n_seqs; a.max_rows = max_rows < T ? max_rows : T; a.T = T;
     a.hold = tl_hold_ns > 0;
     a.wait_ns = a.hold ? tl_hold_ns : PATTN_WAIT_NS;
-    // One of the two for all sequences of a call.  The few-row kernel reads the keys for 8 columns at a time, the wide one makes a tile of 128
-    // whatever it holds: 32 rows of 4096 keys with 8 heads a KV head 21 against 49 us, with 16 columns (two passes' registers) 57 against
-    // 51, 8 rows with 16 heads 32 against 29.  Beside a prompt's rows decode rows cost less in the wide kernel's blocks than two more launches.
+    // One of the two for all sequences of a call.  The few-row kernel reads the keys for 8 columns, the wide one makes a tile of 128
+    // whatever it holds: 32 rows of 4096 keys with 8 heads a KV head 21 us; with 10, 12 and 16 heads over one KV head 41 us in the wide kernel
+    // against 39 to 41 as two calls of half the heads (8 x 16000 keys: 42 against 37 to 39, one row of 4096 keys: 32 against 21 to 23; heads
+    // of 64: 30 against 32 to 33, 30 against 30 to 32, 24 against 18 to 19).
+    // Decode rows beside a prompt's rows are in the wide kernel too: 4 x 1000 keys beside 512 rows behind 2048 positions 49 us, as two calls 59, but 32 x 4096
+    // beside 2048 rows 166 against 142, beside 256 rows 84 against 70, 64 x 2000 beside 1024 rows 120 against 93 (16 heads over 2).
     if ((long long) (n_head / p->n_kv) * a.max_rows <= PATTN_FEW) launch_pattn_few(s, a, tk, tv);
     else launch_pattn_many(s, a, tk, tv);
 }

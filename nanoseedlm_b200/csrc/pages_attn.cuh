@@ -121,7 +121,7 @@ __device__ __forceinline__ void pattn_warm(const PagesAttn& a) {
     const size_t scales = (size_t) a.layer * a.p.n_pages * a.p.n_kv, scale_lines = ((size_t) a.p.n_pages * a.p.n_kv * 4 + 127) / 128;
     const char* const from[5] = {(const char*) a.seqs, (const char*) a.p.table, (const char*) (a.p.ks + scales), (const char*) (a.p.vs + scales), (const char*) a.q};
     const size_t lines[5] = {((size_t) a.n_seqs * sizeof(NslSeqRows) + 127) / 128, ((size_t) a.p.n_seq * a.p.max_pages * 4 + 127) / 128, scale_lines, scale_lines, (((size_t) (a.T - 1) * a.q_stride + (size_t) a.n_head * a.p.hd) * (a.q_type == NSL_BF16 ? 2 : 4) + 127) / 128};
-    const size_t at = (size_t) blockIdx.x * blockDim.x + threadIdx.x;      // one line of each array a thread: 9 MB a launch
+    const size_t at = (size_t) blockIdx.x * blockDim.x + threadIdx.x;      // one line of each array a thread: up to 6 MB of each with 296 blocks of 160
 #pragma unroll
     for (int i = 0; i < 5; ++i)
         if (at < lines[i]) asm volatile("prefetch.global.L2 [%0];" ::"l"(from[i] + 128 * at));

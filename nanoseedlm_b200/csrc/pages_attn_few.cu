@@ -2,7 +2,7 @@
 // head) of a KV head.
 //
 // Bound: HBM, 2 hd + 8 / page bytes a key and KV head (8 x 16001 keys, 8 KV heads over pages of 16: 42 us = 4.0 TB/s; 32 x 4096, 2 KV
-// heads: 20.7 us = 2.4 TB/s, 6.1 between a block's first and last codes).  The step's keys are cut into units of 64 of one (sequence, KV head) and
+// heads: 21.4 us = 2.4 TB/s, 6.1 between a block's first and last codes).  The step's keys are cut into units of 64 of one (sequence, KV head) and
 // dealt evenly to the blocks in order, so a block's units are a few runs of whole pages whatever the lengths.  One warp of a
 // block fetches: page ids and scales 32 pieces ahead, codes by TMA (a piece = a page, or 64 rows of a larger one, swizzled) into
 // a ring.  Four warps compute, 16 keys of the unit each, on the tensor cores with the codes as they are:

@@ -13,10 +13,10 @@
 // two of the four expanded stages at heads of 128 (4096 rows behind 4096 positions: 319 us as bf16 values in f32 arrays, 352 where the call does not say so, 409 with f32 values).
 // The two scales and the running maxima are as in pages_attn_few.cu; here the maxima that the exponents use follow the true ones
 // only when these have grown by 2^8 (weights up to 2^8 then), so O in tensor memory is hardly ever rescaled.
-// Bound: a unit of two tiles takes 1024 clk of exponentials (16 a clock and SM), 1250 clk of products (the second tile's scores read
+// Bound: a unit of two tiles takes 1024 clk of exponentials (16 a clock and SM; 32 more for the factors of its groups' sums, 64 over small pages), 1250 clk of products (the second tile's scores read
 // their A operand from shared memory: 478 instead of 256), about 1300 clk of shared memory (codes in, f16 out, and what the products
 // read) and 1000 issue slots a scheduler; measured 2360, of which 1560 remain without exponentials and most products: the barriers'
-// and loads' latencies of two tiles.  4096 rows behind 4096 positions, 16 heads over 2: 290 us = 711 TFLOP/s.
+// and loads' latencies of two tiles.  4096 rows behind 4096 positions, 16 heads over 2: 292 us = 706 TFLOP/s.
 #include <type_traits>
 
 #include "pages_attn.cuh"
@@ -25,7 +25,7 @@
 namespace nsl {
 
 constexpr int MANY_KEYS = 64, MANY_TILE = 128, MANY_COLS = PATTN_MANY, MANY_THREADS = 480, MANY_RAW = 3, MANY_META = 16;
-constexpr int MANY_EXPAND = 8, MANY_FETCH = 12, MANY_SCORES = 13, MANY_VALUES = 14;      // first warp of each part; the softmax has warps 0 .. 7
+constexpr int MANY_EXPAND = 8, MANY_FETCH = 12, MANY_SCORES = 13;      // first warp of each part; the softmax has warps 0 .. 7, the values' products the last
 constexpr int TM_S = 0, TM_Q = 128, TM_W = 192, TM_O = 256;         // tensor memory columns: S (64 a tile), the first tile's Q (64), W (32 a tile), O (128 a tile)
 constexpr float MANY_SLACK = 8.0f;                                   // how far (in powers of 2) a weight may exceed 1
 
