@@ -94,3 +94,12 @@ def test_known_frequencies_by_parts(rot, scale, factor, values):
 def test_frequencies_of_infinite_arguments(args):
     with pytest.raises(ValueError, match="nsl_rope_freqs"):
         P.rope_freqs(*args)
+
+
+def test_a_status_that_cannot_be_read_is_an_error():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("there is a device to read")
+    L.load().nsl_last_error()
+    assert L.load().nsl_pages_attn_status() == -1
+    assert b"nsl_pages_attn_status" in L.load().nsl_pages_error() and L.last_error() == ""
