@@ -10,7 +10,7 @@
 // soon as the last scores are in registers), 1 the values' (once the weights are there).  An item of up to 128 columns has both
 // tiles work on the same queries, every other unit each, and their states joined at its end.
 // f32 calls (FINE) add the products of the queries' second f16 terms, from shared memory, where an item has any that are not 0; the room for them is
-// two of the four expanded stages at heads of 128 (4096 rows behind 4096 positions: 319 us as bf16 values in f32 arrays, 352 where the call does not say so, 409 with f32 values).
+// a fetched and an expanded stage at heads of 128 (4096 rows behind 4096 positions: 317 us as bf16 values in f32 arrays, 346 where the call does not say so, 383 with f32 values).
 // The two scales and the running maxima are as in pages_attn_few.cu; here the maxima that the exponents use follow the true ones
 // only when these have grown by 2^8 (weights up to 2^8 then), so O in tensor memory is hardly ever rescaled.
 // Bound: a unit of two tiles takes 1024 clk of exponentials (16 a clock and SM; 32 more for the factors of its groups' sums, 64 over small pages), 1250 clk of products (the second tile's scores read
@@ -24,28 +24,29 @@
 
 namespace nsl {
 
-constexpr int MANY_KEYS = 64, MANY_TILE = 128, MANY_COLS = PATTN_MANY, MANY_THREADS = 480, MANY_RAW = 3, MANY_META = 16;
+constexpr int MANY_KEYS = 64, MANY_TILE = 128, MANY_COLS = PATTN_MANY, MANY_THREADS = 480, MANY_META = 16;
 constexpr int MANY_EXPAND = 8, MANY_FETCH = 12, MANY_SCORES = 13;      // first warp of each part; the softmax has warps 0 .. 7, the values' products the last
 constexpr int TM_S = 0, TM_Q = 128, TM_W = 192, TM_O = 256;         // tensor memory columns: S (64 a tile), the first tile's Q (64), W (32 a tile), O (128 a tile)
 constexpr float MANY_SLACK = 8.0f;                                   // how far (in powers of 2) a weight may exceed 1
 
-// FINE: queries as two f16 terms (f32 calls).  The second terms of both tiles take the place of two stages at heads of 128.
+// FINE: queries as two f16 terms (f32 calls).  The second terms of both tiles take the place of a fetched and an expanded stage at heads of 128
+// (of two expanded ones: 352 us where this takes 346, 409 where it takes 383).
 template <int HD, bool FINE>
 struct Many {
-    static constexpr int STAGES = FINE && HD == 128 ? 2 : 4;
+    static constexpr int RAWS = FINE && HD == 128 ? 2 : 3, STAGES = FINE && HD == 128 ? 3 : 4;
     static constexpr int RAW = MANY_KEYS * HD;                       // bytes of a unit's key codes, or value codes
     static constexpr int TILE = 2 * RAW;                             // the same as f16
     static constexpr int QUERIES = 2 * MANY_TILE * HD;               // bytes of a tile's queries as f16
-    static constexpr int OFF_TILES = MANY_RAW * 2 * RAW;
+    static constexpr int OFF_TILES = RAWS * 2 * RAW;
     static constexpr int OFF_Q = OFF_TILES + STAGES * 2 * TILE;      // the second tile's queries
     static constexpr int OFF_QLOW = OFF_Q + QUERIES;                 // FINE: both tiles' second terms
     static constexpr int OFF_META = OFF_QLOW + (FINE ? 2 * QUERIES : 0);
     static constexpr int OFF_BARS = OFF_META + MANY_META * 4 * 16;
-    static constexpr int BARS = 2 * MANY_RAW + 2 * STAGES + MANY_META + 11;
+    static constexpr int BARS = 2 * RAWS + 2 * STAGES + MANY_META + 11;
     static constexpr int SMEM = OFF_BARS + 8 * BARS + 1024;
 };
 static_assert(MANY_COLS == 2 * MANY_TILE, "two tiles an item");
-static_assert(Many<128, false>::SMEM + 2048 <= 232448 && Many<128, true>::SMEM + 2048 <= 232448, "shared memory");
+static_assert(Many<128, false>::SMEM + 256 <= 232448 && Many<128, true>::SMEM + 256 <= 232448, "shared memory");
 constexpr int MANY_SEQS = 4096;      // descriptors of a call; their units sit in the tiles' memory while the plan is made
 static_assert(MANY_SEQS * 4 <= 4 * 4 * 64 * 64, "the plan's memory: four stages at heads of 64, two or four at 128");
 
@@ -152,6 +153,14 @@ __device__ __forceinline__ void tm_st16(uint32_t at, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
                    "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void tm_ld4(uint32_t at, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+    tm_wait_ld();
+}
+__device__ __forceinline__ void tm_st4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -275,23 +284,22 @@ static __device__ __noinline__ void many_results(const PagesAttn& a, uint32_t to
 template <int HD, bool WIDE, bool FINE>
 __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __grid_constant__ PagesAttn a, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
     using F = Many<HD, FINE>;
-    constexpr int STAGES = F::STAGES, STATE = PATTN_STATE<HD>, WARPS = MANY_THREADS / 32, NG = WIDE ? 1 : 4, GK = MANY_KEYS / NG;      // groups of GK keys with one pair of scales
+    constexpr int RAWS = F::RAWS, STAGES = F::STAGES, STATE = PATTN_STATE<HD>, WARPS = MANY_THREADS / 32, NG = WIDE ? 1 : 4, GK = MANY_KEYS / NG;      // groups of GK keys with one pair of scales
     extern __shared__ uint8_t many_raw[];
     uint8_t* const smem = (uint8_t*) (((uintptr_t) many_raw + 1023) & ~(uintptr_t) 1023);
     __shared__ int wsum[WARPS], plan[2], abort_flag;
     __shared__ uint32_t tmem_slot;
     __shared__ int q_low[MANY_EXPAND];      // FINE, by softmax warp: do its columns' queries have second terms that are not 0
-    __shared__ float other[3][MANY_TILE];      // the second tile's m, l, mo where both have the same columns
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.n_head / a.p.n_kv;
     const uint32_t base = pa_smem(smem), tiles = base + F::OFF_TILES, bars = base + F::OFF_BARS;
     // arrivals: raw_full the fetch (and bytes), raw_empty the 4 expanding warps, tile_full the same, tile_empty the products, meta the fetch;
     // per tile: s_full and o_done (a unit's scores are there, its values are in O) the products, s_free (the scores are in registers),
     // w_full and q_full the tile's 4 warps; done the warps that issue products
-    const uint32_t raw_full = bars, raw_empty = raw_full + 8 * MANY_RAW, tile_full = raw_empty + 8 * MANY_RAW, tile_empty = tile_full + 8 * STAGES, meta_full = tile_empty + 8 * STAGES,
+    const uint32_t raw_full = bars, raw_empty = raw_full + 8 * RAWS, tile_full = raw_empty + 8 * RAWS, tile_empty = tile_full + 8 * STAGES, meta_full = tile_empty + 8 * STAGES,
                    s_full = meta_full + 8 * MANY_META, s_free = s_full + 16, w_full = s_free + 16, q_full = w_full + 16, o_done = q_full + 16, done = o_done + 16;
     const float4* const meta = (const float4*) (smem + F::OFF_META);
     if (tid == 0) {
-        for (int i = 0; i < MANY_RAW; ++i) { pa_bar_init(raw_full + 8 * i, 1); pa_bar_init(raw_empty + 8 * i, 4); }
+        for (int i = 0; i < RAWS; ++i) { pa_bar_init(raw_full + 8 * i, 1); pa_bar_init(raw_empty + 8 * i, 4); }
         for (int i = 0; i < STAGES; ++i) { pa_bar_init(tile_full + 8 * i, 4); pa_bar_init(tile_empty + 8 * i, 1); }
         for (int i = 0; i < MANY_META; ++i) pa_bar_init(meta_full + 8 * i, 1);
         for (int t = 0; t < 2; ++t) { pa_bar_init(s_full + 8 * t, 1); pa_bar_init(s_free + 8 * t, 4); pa_bar_init(w_full + 8 * t, 4); pa_bar_init(q_full + 8 * t, 4); pa_bar_init(o_done + 8 * t, 1); }
@@ -498,15 +506,18 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
             // ---- results ----
             const int b0 = it.first / per, parts = (it.first + it.units - 1) / per - b0 + 1;
             float by = 1.0f, by1 = 0.0f;      // what this tile's and the second's O are multiplied with
-            if (shared && t == 1) { other[0][c] = m; other[1][c] = l; other[2][c] = mo; }
-            if (shared) {
+            if (shared) {      // the second tile's m, l, mo by its weights' columns, whose last have been read, to the warp that has the same lanes
+                __syncwarp();
+                if (t == 1) tm_st4(tw, __float_as_uint(m), __float_as_uint(l), __float_as_uint(mo), 0u);
                 tm_before();
                 softmax_sync();
                 tm_after();
                 if (t == 0) {
-                    const float m1 = other[0][c], mo1 = other[2][c], mm = fmaxf(m, m1), mmo = fmaxf(mo, mo1);
+                    uint32_t st[4];
+                    tm_ld4(tw + 32, st);
+                    const float m1 = __uint_as_float(st[0]), mo1 = __uint_as_float(st[2]), mm = fmaxf(m, m1), mmo = fmaxf(mo, mo1);
                     const float ms = mm == -INFINITY ? 0.0f : mm, mos = mmo == -INFINITY ? 0.0f : mmo;
-                    l = l * pa_ex2(m - ms) + other[1][c] * pa_ex2(m1 - ms);
+                    l = l * pa_ex2(m - ms) + __uint_as_float(st[1]) * pa_ex2(m1 - ms);
                     by = pa_ex2(mo - mos);
                     by1 = pa_ex2(mo1 - mos);
                     m = mm;
@@ -539,8 +550,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
         const int odd = lane >> 4, half = lane >> 3 & 1;
         const uint32_t v_to = (uint32_t) F::TILE + (uint32_t) (8 * odd + (lane & 7)) * 128 + (((uint32_t) (2 * w + half) ^ (uint32_t) (lane & 7)) << 4);
         for (int n = xe - x0; g < n; ++g) {
-            const uint32_t rs = (uint32_t) (g % MANY_RAW), st = (uint32_t) (g % STAGES);
-            wait(raw_full + 8 * rs, g / MANY_RAW & 1, 7);
+            const uint32_t rs = (uint32_t) (g % RAWS), st = (uint32_t) (g % STAGES);
+            wait(raw_full + 8 * rs, g / RAWS & 1, 7);
             if (g >= STAGES) wait(tile_empty + 8 * st, (g / STAGES - 1) & 1, 8);
             const uint32_t raw = base + rs * 2 * F::RAW, out = tiles + st * 2 * F::TILE;
             // keys: row and chunk of 16 codes a thread -> two 16-byte pieces of the row's f16 values
@@ -594,8 +605,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
                 }
                 const int row = id < 0 ? -1 : (int) ((head_at + (size_t) id * a.p.n_kv) * a.p.page + p % a.p.page);
                 for (int u = 0; u < batch && b + u < it.x1; ++u, ++g) {
-                    const uint32_t rs = (uint32_t) (g % MANY_RAW);
-                    if (g >= MANY_RAW) wait(raw_empty + 8 * rs, (g / MANY_RAW - 1) & 1, 9);
+                    const uint32_t rs = (uint32_t) (g % RAWS);
+                    if (g >= RAWS) wait(raw_empty + 8 * rs, (g / RAWS - 1) & 1, 9);
                     if (__any_sync(0xFFFFFFFFu, *(volatile int*) &abort_flag)) break;      // by all lanes or none
                     const int from = u * pieces + (lane & (pieces - 1)), of_group = u * pieces + (lane & 3) * 16 / piece;
                     const int my_row = __shfl_sync(0xFFFFFFFFu, row, from), g_row = __shfl_sync(0xFFFFFFFFu, row, of_group);
@@ -616,8 +627,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) pattn_many_kernel(const __gri
                 }
             }
         }
-        for (int i = 0; i < MANY_RAW; ++i) {      // what is in flight ends before the block does, whatever the others do
-            const int filled = g / MANY_RAW + (i < g % MANY_RAW);
+        for (int i = 0; i < RAWS; ++i) {      // what is in flight ends before the block does, whatever the others do
+            const int filled = g / RAWS + (i < g % RAWS);
             if (filled > 0) for (uint32_t k = 0; k < (1u << 20) && !pa_bar_try(raw_full + 8 * i, (filled - 1) & 1); ++k) {}
         }
     } else {      // ---- issues the products: the scores', or the values' ----
