@@ -48,10 +48,10 @@ typedef struct {
  * -> 0, or -1 with a message (rot not even and positive, theta <= 1 or scale < 1 or not finite, or ctx / betas unusable). */
 enum { NSL_ROPE_PLAIN = 0, NSL_ROPE_LINEAR = 1, NSL_ROPE_BASE = 2, NSL_ROPE_PARTS = 3 };
 int nsl_rope_freqs(int kind, int rot, double theta, double scale, int ctx, double beta_fast, double beta_slow, float* inv, float* factor);
-/* Rows of heads rotated: x = factor (u cos a - w sin a, w cos a + u sin a), a = pos[t] * inv[p], the product reduced to a
- * quarter turn with all its bits (the angle is right to 1e-15 for every int32 position, its sine and cosine to 1.2e-10 and a rounding to f32).  q, qo [T][n_head][hd] with row strides in elements, k, ko [T][n_kv][hd]
- * (n_kv = 0: none; n_head = 0: none); outputs may be the inputs; a call whose outputs otherwise overlap
- * them, or one another, is refused.  hd a multiple of 16, at
+/* Rows of heads rotated: x = factor (u cos a - w sin a, w cos a + u sin a), a = pos[t] * inv[p], the product reduced to a quarter
+ * turn with all its bits (for frequencies up to 1 the angle is right to 1e-15 at every int32 position, its sine and cosine to 1.2e-10 and a
+ * rounding to f32).  q, qo [T][n_head][hd] with row strides in elements, k, ko [T][n_kv][hd] (n_kv = 0: none; n_head = 0: none);
+ * outputs may be the inputs; a call whose outputs otherwise overlap them, or one another, is refused.  hd a multiple of 16, at
  * most 512; rows start on 16-byte boundaries. */
 void nsl_rope(cudaStream_t s, NslRope r, int type, int hd, const void* q, int q_stride, void* qo, int qo_stride, int n_head, const void* k, int k_stride,
               void* ko, int ko_stride, int n_kv, const int32_t* pos, int T);
